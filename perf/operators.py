@@ -222,10 +222,10 @@ def prepare(case, seed):
         for r in range(reqs):
             live[r, max(lens[r] - n_q[r] - w + 1, 0) // PAGE:-(-lens[r] // PAGE)] = True
             live[r, :min(-(-sk // PAGE), -(-lens[r] // PAGE))] = True
-        blocks = int(live.sum()) + 1
+        blocks = max(int(live.sum()) + 1, 3)
         live = live.cuda()
         s["table"] = torch.randint(0, blocks, (reqs, wide), generator=gen, device="cuda", dtype=torch.int32)
-        s["table"][live] = torch.randperm(blocks, generator=gen, device="cuda")[:blocks - 1].to(torch.int32)
+        s["table"][live] = torch.randperm(blocks, generator=gen, device="cuda")[:int(live.sum())].to(torch.int32)
         s["cache"] = _cache(gen, blocks, n_kv)
         cu = [0]
         for n in n_q:
@@ -246,7 +246,7 @@ def prepare(case, seed):
                 table[r, whole:whole + m] = torch.arange(n, n + m)
                 n += m
         s["table"] = torch.randperm(n, generator=gen, device="cuda").to(torch.int32)[table.cuda()]
-        s["cache"] = _cache(gen, n, n_kv)
+        s["cache"] = _cache(gen, max(n, 3), n_kv)
         first = torch.tensor(cu[:-1], device="cuda")
         group = torch.bucketize(torch.arange(reqs, device="cuda"), torch.tensor(cu[1:], device="cuda"), right=True)
         # the copied part of a prefix's last page holds the same tokens in every request of the group
