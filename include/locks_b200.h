@@ -50,6 +50,9 @@ extern "C" {
 #define LOCKS_ST_WAIT_TIMEOUT  1  /* a bounded on-chip wait ran out            */
 #define LOCKS_ST_CP_OVERFLOW   2  /* context parallel: more kept pages than     */
                                   /* candidate slots (cap sized too small)      */
+#define LOCKS_ST_PLAN_REFUSED  3  /* append plan: a request did not fit its     */
+                                  /* table row, the free list or the token      */
+                                  /* arrays                                     */
 
 #define LOCKS_COMBINE_NONE 0      /* `score` already holds the combined score  */
 #define LOCKS_COMBINE_NRM  1      /* sum_g exp(S[g,p] - max_p S[g,p])          */
@@ -580,6 +583,94 @@ int locks_dense_decode(const void* q, int64_t q_stride_req, const void* k_cache,
                        int n_req, int n_kv, int G, int head_dim, int page,
                        int split, float scale, int* status,
                        locks_stream_t stream);
+
+/* ---- Serving step around the paged cache ------------------------------------------
+ * No counterparts in the reference, whose engine does these steps elsewhere.
+ * All four: page 16 (append plan: any), head_dim 128, 1 <= G <= 16, bf16 queries,
+ * keys, values and outputs; rows 16-byte aligned (strides multiples of 8).
+ *
+ * locks_append_plan: where the step's new tokens go.  Request r has seq_lens[r]
+ * tokens cached and n_new[r] >= 0 new ones; its table row (bt_width columns) names
+ * the blocks of its cached tokens; free_blocks[*taken .. n_free) are the blocks
+ * that can still be handed out.  In request order, a request whose tokens need
+ * more pages than it has takes the next blocks of the list and they are entered in
+ * its table row.  Outputs: cu_tokens[r] = sum of n_new before r (n_req + 1
+ * entries); per token, in that layout, slot_mapping (block * page + offset) and
+ * positions; lens_out[r] = seq_lens[r] + n_new[r]; *taken_out.  lens_out may be
+ * seq_lens and taken_out may be taken.  Entries of slot_mapping / positions behind
+ * the last token, up to max_tokens, become -1 / 0 (a padded batch).  A request that
+ * does not fit -- its table row, the rest of the free list, or max_tokens -- is
+ * refused as a whole: slots -1, no block, no entry, length unchanged, and *status
+ * (optional) becomes LOCKS_ST_PLAN_REFUSED; later requests that fit are served
+ * as long as they need no block the refused one left short.  n_req <= 4096; the sum
+ * of n_new below 2^31.
+ *
+ * locks_norm_rope_write: RMS norm of every query and key head (w / null: no norm),
+ * rotation of the first rot_dim channels at positions[t] (null cos_sin: none;
+ * half-split or interleaved pairing, table rows cos half then sin half, as
+ * locks_kv_write), q to q_out (which may be q), K and V to the cache at
+ * slot_mapping[t] (negative or beyond the cache: not stored).  fp32 throughout, one
+ * rounding at the end.  Table and weights are bf16 or fp32 (table_f32, weight_f32);
+ * weights have head_dim values.  Positions outside [0, n_positions) read the
+ * nearest table row.  Two tokens with one slot leave either one's rows there.
+ *
+ * locks_window_attention: attention of ragged query runs over the paged cache.
+ * Request r's queries are tokens cu_q[r] .. cu_q[r + 1) of q; it has seq_lens[r]
+ * tokens cached, the new ones among them, so query i sits at position p =
+ * seq_lens[r] - n_q + i and sees key j <= p when p - j < window or j < sinks
+ * (window >= the longest sequence: plain causal attention).  A row that sees
+ * nothing becomes 0 with lse -inf; tokens behind cu_q[n_req] are left as they were.
+ * Pages that no query of a request sees are not read: their table entries may hold
+ * anything.  Keys and values of the seen pages must be finite up to seq_lens[r].
+ * Block ids are clamped to [0, num_blocks), keys end with the table's last column.
+ * lse: optional f32 natural log-sum-exp, lse[token * lse_stride_tok + head].
+ * max_q: no request has more query tokens (a bound the host knows).
+ * scratch: optional fp32 workspace; what the call leaves there is of no use to
+ * anyone, and calls that may overlap on the GPU need one each.
+ *
+ * locks_shared_prefix_decode: one query token per request (row r of q, position
+ * seq_lens[r] - 1), requests [cu_groups[g], cu_groups[g + 1]) share the first
+ * prefix_lens[g] tokens: those tokens are read once for the group, through the
+ * table row of its first request, whole pages only (the page a prefix ends in is
+ * read by each request itself).  Results equal attention of every request over
+ * its own table.  Rows outside the groups are left as they were; a request with
+ * seq_lens[r] <= 0 gets 0.  scratch (fp32, scratch_floats of them): at least
+ * n_req * n_kv * G * (head_dim + 2); more lets a long prefix be cut into more
+ * parts. */
+int locks_append_plan(const int32_t* seq_lens, const int32_t* n_new,
+                      int32_t* block_table, int64_t bt_stride, int bt_width,
+                      const int32_t* free_blocks, int n_free, const int32_t* taken,
+                      int64_t* slot_mapping, int64_t* positions, int32_t* cu_tokens,
+                      int32_t* lens_out, int32_t* taken_out, int n_req,
+                      int max_tokens, int page, int* status, locks_stream_t stream);
+int locks_norm_rope_write(
+    const void* q, int64_t q_stride_tok, int64_t q_stride_head, const void* key,
+    int64_t k_stride_tok, int64_t k_stride_head, const void* val, int64_t v_stride_tok,
+    int64_t v_stride_head, void* q_out, int64_t o_stride_tok, int64_t o_stride_head,
+    void* k_cache, void* v_cache, int64_t kv_stride_block, int64_t kv_stride_tok,
+    int64_t kv_stride_head, const int64_t* slot_mapping, const int64_t* positions,
+    const void* cos_sin, int64_t cos_sin_row_stride, int n_positions, int rot_dim,
+    int neox, int table_f32, const void* q_weight, const void* k_weight, int weight_f32,
+    float eps, int n_tok, int n_heads, int n_kv, int head_dim, int page, int num_blocks,
+    locks_stream_t stream);
+int locks_window_attention(
+    const void* q, int64_t q_stride_tok, int64_t q_stride_head, const void* k_cache,
+    const void* v_cache, int64_t kv_stride_block, int64_t kv_stride_tok,
+    int64_t kv_stride_head, const int32_t* block_table, int64_t bt_stride, int bt_width,
+    int num_blocks, const int32_t* cu_q, const int32_t* seq_lens, void* out,
+    int64_t o_stride_tok, int64_t o_stride_head, float* lse, int64_t lse_stride_tok,
+    float* scratch, int64_t scratch_floats, int n_tok, int n_req, int max_q, int n_kv,
+    int G, int head_dim, int page, int window, int sinks, float scale, int* status,
+    locks_stream_t stream);
+int locks_shared_prefix_decode(
+    const void* q, int64_t q_stride_req, int64_t q_stride_head, const void* k_cache,
+    const void* v_cache, int64_t kv_stride_block, int64_t kv_stride_tok,
+    int64_t kv_stride_head, const int32_t* block_table, int64_t bt_stride, int bt_width,
+    int num_blocks, const int32_t* seq_lens, const int32_t* cu_groups,
+    const int32_t* prefix_lens, void* out, int64_t o_stride_req, int64_t o_stride_head,
+    float* lse, int64_t lse_stride_req, float* scratch, int64_t scratch_floats, int n_req,
+    int n_groups, int n_kv, int G, int head_dim, int page, float scale, int* status,
+    locks_stream_t stream);
 
 /* ---- MLA (latent KV) path ------------------------------------------------
  * Geometry: latent width kv_lora_rank 512 + rope 64 = 576, page 16, 16 query

@@ -1,0 +1,99 @@
+// Entry points of the windowed and the shared-prefix attention over the paged cache.
+#include "common.cuh"
+#include "paged_rows.cuh"
+
+namespace locks {
+namespace {
+
+bool rows16(const void* p, int64_t a, int64_t b) {
+    return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && a % 8 == 0 && b % 8 == 0;
+}
+
+// the checks both entry points share
+int check_paged(const char* who, const RowAttnParams& p, int n_req, int head_dim, int page,
+                const float* scratch, int64_t scratch_floats) {
+    LOCKS_REQUIRE(p.q && p.k && p.v && p.table && p.seq_lens && p.out, LOCKS_ERR_ARG,
+                  "%s: null pointer argument", who);
+    LOCKS_REQUIRE(head_dim == PR_HD && page == PR_PAGE, LOCKS_ERR_GEOMETRY,
+                  "%s: supports head_dim 128 / page 16, got %d / %d", who, head_dim, page);
+    LOCKS_REQUIRE(p.G >= 1 && p.G <= 16, LOCKS_ERR_GEOMETRY,
+                  "%s: supports 1 <= G <= 16, got %d", who, p.G);
+    LOCKS_REQUIRE(n_req >= 0 && n_req <= 65535 && p.n_kv >= 1 && p.n_kv <= 65535 &&
+                      p.bt_width >= 1 && p.bt_width <= (1 << 26) && p.num_blocks >= 1 &&
+                      p.sinks >= 0 && p.window >= 0 && scratch_floats >= 0,
+                  LOCKS_ERR_ARG, "%s: bad size argument", who);
+    LOCKS_REQUIRE(rows16(p.q, p.q_tok, p.q_head) && rows16(p.k, p.st, p.sh) &&
+                      rows16(p.v, p.sb, 0) && rows16(p.out, p.o_tok, p.o_head),
+                  LOCKS_ERR_ARG, "%s: rows must be 16-byte aligned", who);
+    LOCKS_REQUIRE((reinterpret_cast<uintptr_t>(scratch) & 15) == 0, LOCKS_ERR_ARG,
+                  "%s: scratch must be 16-byte aligned", who);
+    return LOCKS_OK;
+}
+
+}  // namespace
+}  // namespace locks
+
+using namespace locks;
+
+extern "C" int locks_window_attention(
+    const void* q, int64_t q_stride_tok, int64_t q_stride_head, const void* k_cache,
+    const void* v_cache, int64_t kv_stride_block, int64_t kv_stride_tok,
+    int64_t kv_stride_head, const int32_t* block_table, int64_t bt_stride, int bt_width,
+    int num_blocks, const int32_t* cu_q, const int32_t* seq_lens, void* out,
+    int64_t o_stride_tok, int64_t o_stride_head, float* lse, int64_t lse_stride_tok,
+    float* scratch, int64_t scratch_floats, int n_tok, int n_req, int max_q, int n_kv,
+    int G, int head_dim, int page, int window, int sinks, float scale, int* status,
+    locks_stream_t stream) {
+    RowAttnParams p = {};
+    p.q = static_cast<const __nv_bfloat16*>(q); p.q_tok = q_stride_tok; p.q_head = q_stride_head;
+    p.k = static_cast<const __nv_bfloat16*>(k_cache);
+    p.v = static_cast<const __nv_bfloat16*>(v_cache);
+    p.sb = kv_stride_block; p.st = kv_stride_tok; p.sh = kv_stride_head;
+    p.table = block_table; p.bt_stride = bt_stride; p.bt_width = bt_width;
+    p.num_blocks = num_blocks; p.cu_q = cu_q; p.seq_lens = seq_lens;
+    p.out = static_cast<__nv_bfloat16*>(out); p.o_tok = o_stride_tok; p.o_head = o_stride_head;
+    p.lse = lse; p.lse_tok = lse_stride_tok;
+    p.n_kv = n_kv; p.G = G; p.window = window; p.sinks = sinks;
+    p.scale_log2 = scale * PR_LOG2E;
+    const char* who = "locks_window_attention";
+    const int rc = check_paged(who, p, n_req, head_dim, page, scratch, scratch_floats);
+    if (rc != LOCKS_OK) return rc;
+    LOCKS_REQUIRE(cu_q, LOCKS_ERR_ARG, "%s: null pointer argument", who);
+    LOCKS_REQUIRE(n_tok >= 0 && max_q >= 0, LOCKS_ERR_ARG, "%s: bad size argument", who);
+    if (n_req == 0 || n_tok == 0 || max_q == 0) return LOCKS_OK;
+    return launch_row_attn(who, p, n_req, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int locks_shared_prefix_decode(
+    const void* q, int64_t q_stride_req, int64_t q_stride_head, const void* k_cache,
+    const void* v_cache, int64_t kv_stride_block, int64_t kv_stride_tok,
+    int64_t kv_stride_head, const int32_t* block_table, int64_t bt_stride, int bt_width,
+    int num_blocks, const int32_t* seq_lens, const int32_t* cu_groups,
+    const int32_t* prefix_lens, void* out, int64_t o_stride_req, int64_t o_stride_head,
+    float* lse, int64_t lse_stride_req, float* scratch, int64_t scratch_floats, int n_req,
+    int n_groups, int n_kv, int G, int head_dim, int page, float scale, int* status,
+    locks_stream_t stream) {
+    RowAttnParams p = {};
+    p.q = static_cast<const __nv_bfloat16*>(q); p.q_tok = q_stride_req; p.q_head = q_stride_head;
+    p.k = static_cast<const __nv_bfloat16*>(k_cache);
+    p.v = static_cast<const __nv_bfloat16*>(v_cache);
+    p.sb = kv_stride_block; p.st = kv_stride_tok; p.sh = kv_stride_head;
+    p.table = block_table; p.bt_stride = bt_stride; p.bt_width = bt_width;
+    p.num_blocks = num_blocks; p.seq_lens = seq_lens;
+    p.out = static_cast<__nv_bfloat16*>(out); p.o_tok = o_stride_req; p.o_head = o_stride_head;
+    p.lse = lse; p.lse_tok = lse_stride_req;
+    p.n_kv = n_kv; p.G = G; p.window = INT32_MAX; p.sinks = 0;
+    p.scale_log2 = scale * PR_LOG2E;
+    p.cu_groups = cu_groups; p.n_groups = n_groups;
+    const char* who = "locks_shared_prefix_decode";
+    const int rc = check_paged(who, p, n_req, head_dim, page, scratch, scratch_floats);
+    if (rc != LOCKS_OK) return rc;
+    LOCKS_REQUIRE(cu_groups && prefix_lens && scratch, LOCKS_ERR_ARG,
+                  "%s: null pointer argument", who);
+    LOCKS_REQUIRE(n_groups >= 0, LOCKS_ERR_ARG, "%s: bad size argument", who);
+    LOCKS_REQUIRE(scratch_floats >= (int64_t)n_req * n_kv * G * (PR_HD + 2), LOCKS_ERR_SIZE,
+                  "%s: scratch holds %lld floats, at least %lld are needed", who,
+                  (long long)scratch_floats, (long long)n_req * n_kv * G * (PR_HD + 2));
+    if (n_req == 0 || n_groups == 0) return LOCKS_OK;
+    return launch_row_attn(who, p, n_req, static_cast<cudaStream_t>(stream));
+}

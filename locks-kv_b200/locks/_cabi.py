@@ -87,6 +87,17 @@ _SIGNATURES = {
     "locks_decode_split_noalloc": ([_P, _L, _P, _P, _L, _L, _L, _P, _L, _P, _P,
                                     _P, _P, _L, _I, _I, _I, _I, _I, _I, _I, _I,
                                     _F, _P, _P], 2),
+    "locks_append_plan": ([_P, _P, _P, _L, _I, _P, _I, _P, _P, _P, _P, _P, _P, _I,
+                           _I, _I, _P, _P], 1),
+    "locks_norm_rope_write": ([_P, _L, _L, _P, _L, _L, _P, _L, _L, _P, _L, _L, _P,
+                               _P, _L, _L, _L, _P, _P, _P, _L, _I, _I, _I, _I, _P,
+                               _P, _I, _F, _I, _I, _I, _I, _I, _I, _P], 1),
+    "locks_window_attention": ([_P, _L, _L, _P, _P, _L, _L, _L, _P, _L, _I, _I, _P,
+                                _P, _P, _L, _L, _P, _L, _P, _L, _I, _I, _I, _I, _I,
+                                _I, _I, _I, _I, _F, _P, _P], 1),
+    "locks_shared_prefix_decode": ([_P, _L, _L, _P, _P, _L, _L, _L, _P, _L, _I, _I,
+                                    _P, _P, _P, _P, _L, _L, _P, _L, _P, _L, _I, _I,
+                                    _I, _I, _I, _I, _F, _P, _P], 1),
     "locks_mla_build_factors": ([_P, _L, _L, _P, _P, _I, _I, _P], 1),
     "locks_mla_refresh_rows": ([_P, _L, _L, _P, _P, _L, _P, _P, _P, _P, _P, _I, _I,
                                 _I, _P], 2),
@@ -176,6 +187,32 @@ class CpLinkDesc(ctypes.Structure):
                 ("n_layers", ctypes.c_int32), ("p0", ctypes.c_int32),
                 ("cap", ctypes.c_int32), ("b_global", ctypes.c_int32),
                 ("sink_loc", ctypes.c_int32), ("nsh_loc", ctypes.c_int32)]
+
+
+def call_on(dev: torch.device, name: str, *args) -> None:
+    """:func:`call` with ``dev`` current and its current stream as the last
+    argument (the tensors of a call need not live on the current device)."""
+    if dev.index == torch.cuda.current_device():
+        call(name, *args, c_void_p(torch.cuda.current_stream(dev).cuda_stream))
+        return
+    with torch.cuda.device(dev):
+        call(name, *args, c_void_p(torch.cuda.current_stream(dev).cuda_stream))
+
+
+def one_device(*tensors) -> torch.device:
+    """The CUDA device all of the tensors (None is passed over) live on."""
+    dev = None
+    for t in tensors:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise RuntimeError("LOCKS B200 kernels need CUDA tensors, got "
+                               f"{t.device}: there is no CPU path")
+        if dev is None:
+            dev = t.device
+        elif t.device != dev:
+            raise RuntimeError(f"tensors on {dev} and {t.device} in one call")
+    return dev
 
 
 def stream() -> c_void_p:
