@@ -30,6 +30,22 @@ int check_paged(const char* who, const RowAttnParams& p, int n_req, int head_dim
     return LOCKS_OK;
 }
 
+// Requests of up to this many rows (query tokens x G) go to the few-row kernel, whose
+// fragments hold 16; above it the tiled kernel takes 128 rows at a time.
+constexpr int FEW_ROWS = 16;
+constexpr int TILE_ROWS = 256, TILE_PAGES = 8;
+
+// How many parts the key tiles are cut into: enough CTAs for the device, at least two
+// tiles a part (one per stream), as many as the scratch has room for.
+int parts_for(int64_t ctas, int64_t key_pages, int64_t part_floats, int64_t scratch_floats) {
+    const int64_t tiles = (key_pages + TILE_PAGES - 1) / TILE_PAGES;
+    int64_t n = sm_count() / (ctas > 0 ? ctas : 1);
+    n = n < tiles / 2 ? n : tiles / 2;
+    const int64_t room = scratch_floats / part_floats;
+    n = n < room ? n : room;
+    return n < 1 ? 1 : (int)n;
+}
+
 }  // namespace
 }  // namespace locks
 
@@ -60,8 +76,38 @@ extern "C" int locks_window_attention(
     if (rc != LOCKS_OK) return rc;
     LOCKS_REQUIRE(cu_q, LOCKS_ERR_ARG, "%s: null pointer argument", who);
     LOCKS_REQUIRE(n_tok >= 0 && max_q >= 0, LOCKS_ERR_ARG, "%s: bad size argument", who);
+    LOCKS_REQUIRE(scale > 0.f, LOCKS_ERR_ARG, "%s: scale must be positive", who);
     if (n_req == 0 || n_tok == 0 || max_q == 0) return LOCKS_OK;
-    return launch_row_attn(who, p, n_req, static_cast<cudaStream_t>(stream));
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    p.max_rows = INT32_MAX;
+    if ((int64_t)max_q * G > FEW_ROWS) {
+        // (how the tokens fall on the requests is known on the device only: an upper
+        // bound of the tiles, CTAs without one return at once)
+        const int64_t rows = (int64_t)n_tok * G;
+        const int64_t many = rows / (FEW_ROWS + 1) < n_req ? rows / (FEW_ROWS + 1) : n_req;
+        int64_t tiles = rows / TILE_ROWS + many;
+        const int64_t most = many * (((int64_t)max_q * G + TILE_ROWS - 1) / TILE_ROWS);
+        tiles = tiles < most ? tiles : most;
+        if (tiles > 0) {
+            TileAttnParams tp = {};
+            tp.r = p;
+            tp.bounds = cu_q; tp.n_seg = n_req; tp.min_rows = FEW_ROWS; tp.status = status;
+            const int64_t span = (int64_t)window + sinks + max_q;
+            const int64_t pages = span / page + 2 < bt_width ? span / page + 2 : bt_width;
+            p.max_rows = FEW_ROWS;
+            tp.part_rows = (int64_t)n_tok * n_kv * G;
+            tp.parts = scratch ? parts_for(tiles * n_kv, pages, tp.part_rows * (PR_HD + 2),
+                                           scratch_floats) : 1;
+            if (tp.parts > 1) {
+                tp.parts_out = scratch;
+                tp.parts_ml = scratch + tp.parts * tp.part_rows * PR_HD;
+            }
+            int rc2 = launch_tile_attn(who, tp, (int)tiles, s);
+            if (rc2 == LOCKS_OK && tp.parts > 1) rc2 = launch_join_parts(who, tp, n_tok, s);
+            if (rc2 != LOCKS_OK) return rc2;
+        }
+    }
+    return launch_row_attn(who, p, n_req, s);
 }
 
 extern "C" int locks_shared_prefix_decode(
@@ -84,7 +130,7 @@ extern "C" int locks_shared_prefix_decode(
     p.lse = lse; p.lse_tok = lse_stride_req;
     p.n_kv = n_kv; p.G = G; p.window = INT32_MAX; p.sinks = 0;
     p.scale_log2 = scale * PR_LOG2E;
-    p.cu_groups = cu_groups; p.n_groups = n_groups;
+    p.cu_groups = cu_groups; p.n_groups = n_groups; p.prefix_lens = prefix_lens;
     const char* who = "locks_shared_prefix_decode";
     const int rc = check_paged(who, p, n_req, head_dim, page, scratch, scratch_floats);
     if (rc != LOCKS_OK) return rc;
@@ -94,6 +140,22 @@ extern "C" int locks_shared_prefix_decode(
     LOCKS_REQUIRE(scratch_floats >= (int64_t)n_req * n_kv * G * (PR_HD + 2), LOCKS_ERR_SIZE,
                   "%s: scratch holds %lld floats, at least %lld are needed", who,
                   (long long)scratch_floats, (long long)n_req * n_kv * G * (PR_HD + 2));
+    LOCKS_REQUIRE(scale > 0.f, LOCKS_ERR_ARG, "%s: scale must be positive", who);
     if (n_req == 0 || n_groups == 0) return LOCKS_OK;
-    return launch_row_attn(who, p, n_req, static_cast<cudaStream_t>(stream));
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    TileAttnParams tp = {};
+    tp.r = p;
+    tp.bounds = cu_groups; tp.prefix_lens = prefix_lens; tp.n_seg = n_groups;
+    tp.status = status;
+    const int64_t tiles = (int64_t)n_req * G / TILE_ROWS + (n_groups < n_req ? n_groups : n_req);
+    tp.part_rows = (int64_t)n_req * n_kv * G;
+    tp.parts = parts_for(tiles * n_kv, bt_width, tp.part_rows * (PR_HD + 2), scratch_floats);
+    tp.parts_out = scratch;
+    tp.parts_ml = scratch + tp.parts * tp.part_rows * PR_HD;
+    const int rc2 = launch_tile_attn(who, tp, (int)tiles, s);
+    if (rc2 != LOCKS_OK) return rc2;
+    p.max_rows = FEW_ROWS;
+    p.parts = tp.parts; p.part_rows = tp.part_rows;
+    p.parts_o = tp.parts_out; p.parts_ml = tp.parts_ml;
+    return launch_row_attn(who, p, n_req, s);
 }

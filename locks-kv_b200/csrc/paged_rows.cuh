@@ -38,8 +38,9 @@ struct PageList {
     }
 };
 
+// skip: pages before this one are somebody else's business (sinks then 0)
 __device__ __forceinline__ PageList page_list(int pos_lo, int pos_hi, int window, int sinks,
-                                              int bt_width) {
+                                              int bt_width, int skip = 0) {
     PageList l;
     l.pos_lo = pos_lo; l.pos_hi = pos_hi; l.window = window; l.sinks = sinks;
     l.key_end = bt_width * PR_PAGE;
@@ -48,12 +49,38 @@ __device__ __forceinline__ PageList page_list(int pos_lo, int pos_hi, int window
     l.n_first = min((min(sinks, l.key_end) + PR_PAGE - 1) / PR_PAGE, n_pages);
     // first key in the first query's window, rounded down to its page
     const int lo_key = window > pos_lo ? 0 : pos_lo - window + 1;
-    const int from = max(lo_key / PR_PAGE, l.n_first);
+    const int from = max(max(lo_key / PR_PAGE, l.n_first), skip);
     // window 0: nobody's window holds a key
     const int recent = window > 0 ? max(n_pages - from, 0) : 0;
     l.shift = from - l.n_first;
     l.n = l.n_first + recent;
     return l;
+}
+
+// Row `at` of several partial results: channels d .. d + 3 of O, with the maximum (in
+// log2 units) and the sum.  A part that saw nothing carries l = 0 and no O.
+struct PartSum {
+    float m, l;
+    float4 o;
+};
+__device__ __forceinline__ PartSum join_parts(const float* o, const float* ml, int64_t rows,
+                                              int parts, int64_t at, int d) {
+    PartSum r = {-INFINITY, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
+#pragma unroll 4
+    for (int s = 0; s < parts; ++s) {
+        const int64_t i = s * rows + at;
+        const float2 x = *reinterpret_cast<const float2*>(ml + 2 * i);
+        if (x.y > 0.f) {
+            const float4 v = *reinterpret_cast<const float4*>(o + i * PR_HD + d);
+            const float up = fmaxf(r.m, x.x);
+            const float a = pr_exp2(r.m - up), b = pr_exp2(x.x - up);
+            r.l = a * r.l + b * x.y;
+            r.o.x = a * r.o.x + b * v.x; r.o.y = a * r.o.y + b * v.y;
+            r.o.z = a * r.o.z + b * v.z; r.o.w = a * r.o.w + b * v.w;
+            r.m = up;
+        }
+    }
+    return r;
 }
 #endif
 
@@ -73,11 +100,34 @@ struct RowAttnParams {
     int64_t lse_tok;
     int n_kv, G, window, sinks;
     float scale_log2;                 // softmax scale * log2(e)
-    const int32_t* cu_groups;         // shared prefix: (n_groups + 1) row bounds, or null
-    int n_groups;
+    int max_rows;                     // requests with more rows (tokens x G) are left out
+    // shared prefix: (n_groups + 1) row bounds, or null; the whole pages of the prefix
+    // are in `parts` partial results already (layout: TileAttnParams)
+    const int32_t* cu_groups;
+    const int32_t* prefix_lens;
+    int n_groups, parts;
+    int64_t part_rows;
+    const float *parts_o, *parts_ml;
+};
+
+// the tiled kernel: segments bounds[s] .. bounds[s + 1] of query tokens
+struct TileAttnParams {
+    RowAttnParams r;
+    const int32_t* bounds;            // cu_q, or cu_groups of a shared prefix
+    const int32_t* prefix_lens;       // shared prefix: tokens of the segment's prefix
+    int n_seg, min_rows;              // windowed: segments of up to min_rows rows are left out
+    // key tiles cut into `parts`: O relative to its maximum (parts, part_rows, 128) and
+    // (maximum in log2 units, sum) pairs (parts, part_rows, 2); null: one part, final
+    int parts;
+    int64_t part_rows;
+    float *parts_out, *parts_ml;
+    int* status;
 };
 
 // csrc/row_attn.cu; `who` names the entry point in error messages
 int launch_row_attn(const char* who, const RowAttnParams& p, int n_req, cudaStream_t s);
+// csrc/tile_attn.cu
+int launch_tile_attn(const char* who, const TileAttnParams& p, int max_tiles, cudaStream_t s);
+int launch_join_parts(const char* who, const TileAttnParams& p, int n_tok, cudaStream_t s);
 
 }  // namespace locks

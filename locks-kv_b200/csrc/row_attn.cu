@@ -72,11 +72,21 @@ __global__ void __launch_bounds__(RTHREADS) row_attn_kernel(const RowAttnParams 
     const int gid = lane >> 2, tig = lane & 3;
     const int G = p.G;
     // shared prefix: rows that belong to no group are left as they were
-    if (p.cu_groups && (r < p.cu_groups[0] || r >= p.cu_groups[p.n_groups])) return;
+    int skip = 0;                             // whole prefix pages, attended already
+    if (p.cu_groups) {
+        if (r < p.cu_groups[0] || r >= p.cu_groups[p.n_groups]) return;
+        int lo = 0, hi = p.n_groups - 1;
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (p.cu_groups[mid + 1] > r) hi = mid; else lo = mid + 1;
+        }
+        skip = min(max(p.prefix_lens[lo], 0) / PR_PAGE, p.bt_width);
+    }
     const int tok0 = p.cu_q ? p.cu_q[r] : r;
     const int n_q = p.cu_q ? p.cu_q[r + 1] - tok0 : 1;
     const int len = p.seq_lens[r];
     const int rows = n_q * G;
+    if (rows > p.max_rows) return;            // the tiled kernel's
     const int32_t* table = p.table + (int64_t)r * p.bt_stride;
 
     // (the loop bound is the same for every CTA of the cluster)
@@ -87,7 +97,7 @@ __global__ void __launch_bounds__(RTHREADS) row_attn_kernel(const RowAttnParams 
         const int pos_a = len - n_q + min(row_a, rows - 1) / G;
         const int pos_b = len - n_q + min(row_b, rows - 1) / G;
         const PageList list = page_list(len - n_q + i_first, len - n_q + i_last, p.window,
-                                        p.sinks, p.bt_width);
+                                        p.sinks, p.bt_width, skip);
         const int stride = RW * CL, first = c * RW + warp;
         const int n_mine = list.n > first ? (list.n - first + stride - 1) / stride : 0;
 
@@ -276,6 +286,22 @@ __global__ void __launch_bounds__(RTHREADS) row_attn_kernel(const RowAttnParams 
                 o += wt * sm.xacc[cc * per_e + (e - c * per_e)];
             }
             const int at = rb * 16 + row, i = at / G, h = kh * G + at - i * G;
+            if (p.parts) {
+                // (one query token per request: i == 0, tok0 == r)
+                const int64_t pr = (int64_t)tok0 * p.n_kv * G + h;
+#pragma unroll 4
+                for (int s = 0; s < p.parts; ++s) {
+                    const int64_t x = s * p.part_rows + pr;
+                    const float2 ml = *reinterpret_cast<const float2*>(p.parts_ml + 2 * x);
+                    if (ml.y > 0.f) {
+                        const float up = fmaxf(M, ml.x);
+                        const float a = L > 0.f ? pr_exp2(M - up) : 0.f, b = pr_exp2(ml.x - up);
+                        L = a * L + b * ml.y;
+                        o = a * o + b * p.parts_o[x * PR_HD + d];
+                        M = up;
+                    }
+                }
+            }
             p.out[(int64_t)(tok0 + i) * p.o_tok + (int64_t)h * p.o_head + d] =
                 __float2bfloat16_rn(L > 0.f ? o / L : 0.f);
             if (d == 0 && p.lse)
