@@ -64,6 +64,28 @@ struct __align__(1024) TileSmem {
 };
 static_assert(sizeof(TileSmem) + 1024 <= 232448, "one CTA's shared memory");
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+// two fp32 operations in one instruction
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;"
+        : "=l"(reinterpret_cast<uint64_t&>(d))
+        : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)),
+          "l"(reinterpret_cast<uint64_t&>(c)));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("add.rn.f32x2 %0, %1, %2;"
+        : "=l"(reinterpret_cast<uint64_t&>(d))
+        : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+    return d;
+}
+
 // a wait that gives up once any wait of the CTA has
 __device__ __forceinline__ void ta_wait(TileSmem& sm, uint64_t* bar, uint32_t parity,
                                         int* status) {
@@ -329,7 +351,7 @@ tile_attn_kernel(const __grid_constant__ CUtensorMap map_k,
                 }
             }
         }
-    } else {
+    } else if (warp < 8) {
         // ---- softmax: stream i, thread = row ---------------------------------------
         const int i = warp >> 2, q4 = warp & 3;
         const int local = (by_rows ? i * TA_TILE : 0) + q4 * 32 + lane;
@@ -383,8 +405,12 @@ tile_attn_kernel(const __grid_constant__ CUtensorMap map_k,
             }
             float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-            for (int c = 4; c < TA_TILE; ++c) mx[c & 3] = fmaxf(mx[c & 3], s[c]);
-            const float tile_max = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+            for (int c = 4; c < TA_TILE - 4; c += 8)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], s[c + e], s[c + 4 + e]);
+            const float tile_max =
+                fmaxf(max3(max3(mx[0], mx[1], mx[2]), mx[3], s[TA_TILE - 4]),
+                      max3(s[TA_TILE - 3], s[TA_TILE - 2], s[TA_TILE - 1]));
             if (t == 0) {
                 m = tile_max;
             } else if (__any_sync(0xffffffffu, (tile_max - m) * sl2 > TA_RAISE)) {
@@ -397,32 +423,33 @@ tile_attn_kernel(const __grid_constant__ CUtensorMap map_k,
                 __syncwarp();
                 tc_after_sync();
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    uint32_t o[32];
-                    tc_ld32(to + 32 * c, o);
+                for (int c = 0; c < 8; ++c) {
+                    uint32_t o[16];
+                    tc_ld16(to + 16 * c, o);
                     tc_wait_ld();
 #pragma unroll
-                    for (int e = 0; e < 32; ++e)
+                    for (int e = 0; e < 16; ++e)
                         o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                    tc_st32(to + 32 * c, o);
+                    tc_st16(to + 16 * c, o);
                 }
             }
             const float base = m == -INFINITY ? 0.f : m * sl2;
-            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+            const float2 k2 = make_float2(sl2, sl2), b2 = make_float2(-base, -base);
+            float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                uint32_t pk[32];
+            for (int c = 0; c < 4; ++c) {
+                uint32_t pk[16];
 #pragma unroll
-                for (int e = 0; e < 32; ++e) {
-                    const float a = pr_exp2(fmaf(s[64 * c + 2 * e], sl2, -base));
-                    const float b = pr_exp2(fmaf(s[64 * c + 2 * e + 1], sl2, -base));
-                    sum[(2 * e) & 3] += a;
-                    sum[(2 * e + 1) & 3] += b;
-                    pk[e] = pack_bf16x2(a, b);
+                for (int e = 0; e < 16; ++e) {
+                    float2 x = fma2(make_float2(s[32 * c + 2 * e], s[32 * c + 2 * e + 1]), k2, b2);
+                    x.x = pr_exp2(x.x);
+                    x.y = pr_exp2(x.y);
+                    sum[e & 1] = add2(sum[e & 1], x);
+                    pk[e] = pack_bf16x2(x.x, x.y);
                 }
-                tc_st32(ts + 32 * c, pk);
+                tc_st16(ts + 16 * c, pk);
             }
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
             tc_wait_st();
             tc_before_sync();
             __syncwarp();
