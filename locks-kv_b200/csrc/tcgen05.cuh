@@ -6,6 +6,17 @@
 namespace locks {
 
 #ifdef __CUDACC__
+// One lane of a converged warp (warp-uniform code with this predicate keeps matrix
+// descriptors in uniform registers; a lane-number test does not).
+__device__ __forceinline__ bool tc_elect() {
+    uint32_t p;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(p));
+    return p != 0;
+}
 // shared-memory matrix descriptor, 128-byte swizzle, version 1.  K-major operands
 // ([rows][128 B] tiles): sbo = bytes between 8-row groups, lbo unused.  MN-major
 // ([k][64 channels] tiles): lbo = bytes between 64-channel tiles, sbo between

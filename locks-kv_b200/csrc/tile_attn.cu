@@ -161,7 +161,8 @@ tile_attn_kernel(const __grid_constant__ CUtensorMap map_k,
     extern __shared__ uint8_t ta_raw[];
     TileSmem& sm = *reinterpret_cast<TileSmem*>(
         ta_raw + ((1024u - (smem_u32(ta_raw) & 1023u)) & 1023u));
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int tid = threadIdx.x, lane = tid & 31;
+    const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);      // uniform, and known to be
     const int kh = blockIdx.y, part = blockIdx.z, G = p.r.G;
     if (!find_tile(sm, p, blockIdx.x)) return;
     const int seg = sm.seg, row0 = sm.seg_tile * 2 * TA_TILE;
@@ -282,42 +283,57 @@ tile_attn_kernel(const __grid_constant__ CUtensorMap map_k,
                 mbar_wait(&sm.full[i % TA_RING], (uint32_t)(i / TA_RING) & 1u, p.status);
     } else if (warp == 8) {
         // ---- products -------------------------------------------------------------
-        if (lane == 0 && n_tiles > 0) {
+        if (n_tiles > 0) {
             constexpr uint32_t ID_S = tc_idesc(TA_TILE, false), ID_O = tc_idesc(PR_HD, true);
+            const uint64_t desc_q = tc_desc(smem_u32(sm.q), 16, 1024),
+                           desc_k = tc_desc(smem_u32(sm.ring), 16, 1024),
+                           desc_v = tc_desc(smem_u32(sm.ring), TA_HALF, 1024);
             int slot = 0, taken = 0;
             auto take = [&]() {                     // the next tile of the ring
                 const int s = slot;
                 ta_wait(sm, &sm.full[s], (uint32_t)(taken / TA_RING) & 1u, p.status);
+                __syncwarp();
                 slot = slot + 1 == TA_RING ? 0 : slot + 1;
                 ++taken;
                 return s;
             };
             auto scores = [&](int i, int s) {
                 tc_after_sync();
-                const uint64_t a = tc_desc(smem_u32(sm.q[by_rows ? i : 0]), 16, 1024);
-                const uint64_t b = tc_desc(smem_u32(sm.ring[s]), 16, 1024);
+                const uint64_t a = desc_q + (uint64_t)((by_rows ? i : 0) * (TA_BYTES >> 4));
+                const uint64_t b = desc_k + (uint64_t)(s * (TA_BYTES >> 4));
+                if (tc_elect()) {
 #pragma unroll
-                for (int ks = 0; ks < 8; ++ks) {
-                    const uint64_t off = (uint64_t)(((ks >> 2) * TA_HALF + (ks & 3) * 32) >> 4);
-                    tc_mma_ss(tmem + TM_S + i * TA_TILE, a + off, b + off, ID_S, ks ? 1u : 0u);
+                    for (int ks = 0; ks < 8; ++ks) {
+                        const uint64_t off = (uint64_t)(((ks >> 2) * TA_HALF + (ks & 3) * 32) >> 4);
+                        tc_mma_ss(tmem + TM_S + i * TA_TILE, a + off, b + off, ID_S, ks ? 1u : 0u);
+                    }
+                    tc_commit(&sm.s_full[i]);
                 }
-                tc_commit(&sm.s_full[i]);
+                __syncwarp();
             };
             auto values = [&](int i, int s, int t) { // stream i's tile number t
                 ta_wait(sm, &sm.p_ready[i], (uint32_t)t & 1u, p.status);
+                __syncwarp();
                 tc_after_sync();
-                const uint64_t b = tc_desc(smem_u32(sm.ring[s]), TA_HALF, 1024);
+                const uint64_t b = desc_v + (uint64_t)(s * (TA_BYTES >> 4));
+                if (tc_elect()) {
 #pragma unroll
-                for (int ks = 0; ks < TA_PAGES; ++ks)
-                    tc_mma_ts(tmem + TM_O + i * PR_HD, tmem + TM_S + i * TA_TILE + ks * 8,
-                              b + (uint64_t)((ks * TA_BOX) >> 4), ID_O, (t | ks) ? 1u : 0u);
-                tc_commit(&sm.o_full[i]);
+                    for (int ks = 0; ks < TA_PAGES; ++ks)
+                        tc_mma_ts(tmem + TM_O + i * PR_HD, tmem + TM_S + i * TA_TILE + ks * 8,
+                                  b + (uint64_t)((ks * TA_BOX) >> 4), ID_O, (t | ks) ? 1u : 0u);
+                    tc_commit(&sm.o_full[i]);
+                }
+                __syncwarp();
+            };
+            auto release = [&](int s) {
+                if (tc_elect()) tc_commit(&sm.empty[s]);
+                __syncwarp();
             };
             int k_slot = take();
             scores(0, k_slot);
             if (by_rows) {
                 scores(1, k_slot);
-                tc_commit(&sm.empty[k_slot]);
+                release(k_slot);
                 for (int j = 0; j < n_tiles; ++j) {
                     const int v_slot = take();
                     values(0, v_slot, j);
@@ -326,27 +342,27 @@ tile_attn_kernel(const __grid_constant__ CUtensorMap map_k,
                         scores(0, k_slot);
                     }
                     values(1, v_slot, j);
-                    tc_commit(&sm.empty[v_slot]);
+                    release(v_slot);
                     if (j + 1 < n_tiles) {
                         scores(1, k_slot);
-                        tc_commit(&sm.empty[k_slot]);
+                        release(k_slot);
                     }
                 }
             } else {
-                tc_commit(&sm.empty[k_slot]);
+                release(k_slot);
                 if (n_tiles > 1) {
                     k_slot = take();
                     scores(1, k_slot);
-                    tc_commit(&sm.empty[k_slot]);
+                    release(k_slot);
                 }
                 for (int j = 0; j < n_tiles; ++j) {
                     const int v_slot = take();
                     values(j & 1, v_slot, j >> 1);
-                    tc_commit(&sm.empty[v_slot]);
+                    release(v_slot);
                     if (j + 2 < n_tiles) {
                         k_slot = take();
                         scores(j & 1, k_slot);
-                        tc_commit(&sm.empty[k_slot]);
+                        release(k_slot);
                     }
                 }
             }
