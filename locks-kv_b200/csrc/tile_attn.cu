@@ -55,7 +55,7 @@ struct __align__(1024) TileSmem {
     uint8_t q[2][TA_BYTES];
     uint8_t ring[TA_RING][TA_BYTES];
     uint64_t full[TA_RING], empty[TA_RING], tail;
-    uint64_t s_full[2], p_ready[2], o_full[2];
+    uint64_t q_full, s_full[2], p_ready[2], o_full[2];
     uint32_t tmem_base;
     int dead;
     int scan[TA_THREADS / 32];
@@ -101,6 +101,11 @@ __device__ __forceinline__ void ta_wait(TileSmem& sm, uint64_t* bar, uint32_t pa
     if (status) atomicExch(status, LOCKS_ST_WAIT_TIMEOUT);
 }
 
+// 16 bytes global -> shared; src_bytes 0: zeros, nothing is read
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int src_bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
+                 ::"r"(dst), "l"(src), "r"(src_bytes) : "memory");
+}
 __device__ __forceinline__ void tma_load_page(void* dst, const CUtensorMap* map, int channel,
                                               int head, int block, uint64_t* bar) {
     asm volatile(
@@ -197,6 +202,7 @@ tile_attn_kernel(const __grid_constant__ CUtensorMap map_k,
         sm.dead = 0;
         for (int i = 0; i < TA_RING; ++i) { mbar_init(&sm.full[i], 1); mbar_init(&sm.empty[i], 1); }
         mbar_init(&sm.tail, 1);
+        mbar_init(&sm.q_full, 8);
         for (int i = 0; i < 2; ++i) {
             mbar_init(&sm.s_full[i], 1);
             mbar_init(&sm.p_ready[i], 4);
@@ -210,20 +216,6 @@ tile_attn_kernel(const __grid_constant__ CUtensorMap map_k,
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
         tc_before_sync();
     }
-    // Q into the swizzled K-major layout, 16 lanes to a row
-    for (int e = tid; e < (by_rows ? 2 : 1) * TA_TILE * 16; e += TA_THREADS) {
-        const int row = e >> 4, piece = e & 15, at = row0 + row;
-        uint4 x = make_uint4(0, 0, 0, 0);
-        if (row < n_rows) {
-            const int i = at / G;
-            x = *reinterpret_cast<const uint4*>(p.r.q + (int64_t)(t0 + i) * p.r.q_tok +
-                                                (int64_t)(kh * G + at - i * G) * p.r.q_head +
-                                                8 * piece);
-        }
-        *reinterpret_cast<uint4*>(&sm.q[row >> 7][(piece >> 3) * TA_HALF +
-                                                  tc_swz(row & 127, (piece & 7) << 4)]) = x;
-    }
-    fence_proxy_async();
     __syncthreads();
     tc_after_sync();
     const uint32_t tmem = sm.tmem_base;
@@ -330,6 +322,8 @@ tile_attn_kernel(const __grid_constant__ CUtensorMap map_k,
                 __syncwarp();
             };
             int k_slot = take();
+            ta_wait(sm, &sm.q_full, 0, p.status);
+            __syncwarp();
             scores(0, k_slot);
             if (by_rows) {
                 scores(1, k_slot);
@@ -368,6 +362,27 @@ tile_attn_kernel(const __grid_constant__ CUtensorMap map_k,
             }
         }
     } else if (warp < 8) {
+        // ---- Q into the swizzled K-major layout, 16 lanes to a row -------------------
+        {
+            // (rows behind the last one are zeros; every copy is on its way before the
+            // first is waited for)
+            const int piece = tid & 15;
+#pragma unroll 8
+            for (int k = 0; k < (by_rows ? 16 : 8); ++k) {
+                const int row = (tid >> 4) + 16 * k, at = row0 + min(row, n_rows - 1);
+                const int tok = at / G;
+                const __nv_bfloat16* src = p.r.q + (int64_t)(t0 + tok) * p.r.q_tok +
+                                           (int64_t)(kh * G + at - tok * G) * p.r.q_head +
+                                           8 * piece;
+                cp_async16(smem_u32(&sm.q[row >> 7][(piece >> 3) * TA_HALF +
+                                                    tc_swz(row & 127, (piece & 7) << 4)]),
+                           src, row < n_rows ? 16 : 0);
+            }
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sm.q_full);
+        }
         // ---- softmax: stream i, thread = row ---------------------------------------
         const int i = warp >> 2, q4 = warp & 3;
         const int local = (by_rows ? i * TA_TILE : 0) + q4 * 32 + lane;
