@@ -587,7 +587,8 @@ int locks_dense_decode(const void* q, int64_t q_stride_req, const void* k_cache,
 /* ---- Serving step around the paged cache ------------------------------------------
  * No counterparts in the reference, whose engine does these steps elsewhere.
  * All four: page 16 (append plan: any), head_dim 128, 1 <= G <= 16, bf16 queries,
- * keys, values and outputs; rows 16-byte aligned (strides multiples of 8).
+ * keys, values and outputs; rows 16-byte aligned (strides multiples of 8; the two
+ * attentions: the cache's head stride a multiple of 64).
  *
  * locks_append_plan: where the step's new tokens go.  Request r has seq_lens[r]
  * tokens cached and n_new[r] >= 0 new ones; its table row (bt_width columns) names

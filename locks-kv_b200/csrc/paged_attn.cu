@@ -25,6 +25,9 @@ int check_paged(const char* who, const RowAttnParams& p, int n_req, int head_dim
     LOCKS_REQUIRE(rows16(p.q, p.q_tok, p.q_head) && rows16(p.k, p.st, p.sh) &&
                       rows16(p.v, p.sb, 0) && rows16(p.out, p.o_tok, p.o_head),
                   LOCKS_ERR_ARG, "%s: rows must be 16-byte aligned", who);
+    LOCKS_REQUIRE(p.n_kv == 1 || (p.sh % 64 == 0 && p.sh > 0 && p.sh < ((int64_t)1 << 30)),
+                  LOCKS_ERR_GEOMETRY, "%s: the head stride must be a multiple of 64", who);
+    LOCKS_REQUIRE(p.st > 0 && p.sb > 0, LOCKS_ERR_ARG, "%s: bad cache stride", who);
     LOCKS_REQUIRE((reinterpret_cast<uintptr_t>(scratch) & 15) == 0, LOCKS_ERR_ARG,
                   "%s: scratch must be 16-byte aligned", who);
     return LOCKS_OK;

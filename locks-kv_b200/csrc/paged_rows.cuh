@@ -122,12 +122,13 @@ struct TileAttnParams {
     int64_t part_rows;
     float *parts_out, *parts_ml;
     int* status;
+    int head_chunks;                  // 64-channel chunks between two heads
 };
 
 // csrc/row_attn.cu; `who` names the entry point in error messages
 int launch_row_attn(const char* who, const RowAttnParams& p, int n_req, cudaStream_t s);
 // csrc/tile_attn.cu
-int launch_tile_attn(const char* who, const TileAttnParams& p, int max_tiles, cudaStream_t s);
+int launch_tile_attn(const char* who, TileAttnParams p, int max_tiles, cudaStream_t s);
 int launch_join_parts(const char* who, const TileAttnParams& p, int n_tok, cudaStream_t s);
 
 }  // namespace locks

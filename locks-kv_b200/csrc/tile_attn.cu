@@ -47,7 +47,7 @@ constexpr int TA_TILE = 128;                       // keys of a tile, rows of a 
 constexpr int TA_PAGES = TA_TILE / PR_PAGE;
 constexpr int TA_HALF = TA_TILE * 128;             // bytes: 128 rows x 64 channels
 constexpr int TA_BYTES = 2 * TA_HALF;
-constexpr int TA_BOX = PR_PAGE * 128;
+constexpr int TA_BOX = PR_PAGE * 256;              // bytes of a page of one plane and head
 constexpr int TM_S = 0, TM_O = 256, TM_COLS = 512;
 constexpr float TA_RAISE = 8.f;
 
@@ -106,13 +106,16 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int sr
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
                  ::"r"(dst), "l"(src), "r"(src_bytes) : "memory");
 }
-__device__ __forceinline__ void tma_load_page(void* dst, const CUtensorMap* map, int channel,
-                                              int head, int block, uint64_t* bar) {
+// One box = one page of a head: [token / 8][channel / 64][token % 8][64 channels], so
+// that a tile of pages has its groups of 8 keys 2 KiB apart throughout (one box per page
+// instead of one per 64 channels: the copy engine takes about 35 ns for a box of either
+// size, and the tile loop would wait for it).
+__device__ __forceinline__ void tma_load_page(void* dst, const CUtensorMap* map, int chunk,
+                                              int block, uint64_t* bar) {
     asm volatile(
-        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes "
-        "[%0], [%1, {%2, %3, %4, %5}], [%6];"
-        ::"r"(smem_u32(dst)), "l"(map), "r"(channel), "r"(head), "r"(0), "r"(block),
-          "r"(smem_u32(bar))
+        "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes "
+        "[%0], [%1, {%2, %2, %3, %2, %4}], [%5];"
+        ::"r"(smem_u32(dst)), "l"(map), "r"(0), "r"(chunk), "r"(block), "r"(smem_u32(bar))
         : "memory");
 }
 
@@ -240,9 +243,9 @@ tile_attn_kernel(const __grid_constant__ CUtensorMap map_k,
             uint64_t* bar = cut ? &sm.tail : &sm.full[slot];
             if (lane == 0) mbar_expect_tx(bar, TA_BYTES);
             __syncwarp();
-            if (lane < 16)
-                tma_load_page(&sm.ring[slot][(lane >> 3) * TA_HALF + (lane & 7) * TA_BOX],
-                              is_v ? &map_v : &map_k, 64 * (lane >> 3), kh, blk, bar);
+            if (lane < TA_PAGES)
+                tma_load_page(&sm.ring[slot][lane * TA_BOX], is_v ? &map_v : &map_k,
+                              kh * p.head_chunks, blk, bar);
             if (cut) {
                 // the sequence ends inside a page: what the cache holds behind it may
                 // be anything, and 0 x NaN is not 0
@@ -252,9 +255,9 @@ tile_attn_kernel(const __grid_constant__ CUtensorMap map_k,
                 const int from = max(written - __shfl_sync(0xffffffffu, page, s) * PR_PAGE, 0);
                 for (int e = lane; e < (PR_PAGE - from) * 16; e += 32)
                     *reinterpret_cast<uint4*>(
-                        &sm.ring[slot][((e >> 3) & 1) * TA_HALF + s * TA_BOX +
-                                       (from + (e >> 4)) * 128 + (e & 7) * 16]) =
-                        make_uint4(0, 0, 0, 0);
+                        &sm.ring[slot][s * TA_BOX + ((from + (e >> 4)) >> 3) * 2048 +
+                                       ((e >> 3) & 1) * 1024 + ((from + (e >> 4)) & 7) * 128 +
+                                       (e & 7) * 16]) = make_uint4(0, 0, 0, 0);
                 fence_proxy_async();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sm.full[slot]);
@@ -278,8 +281,8 @@ tile_attn_kernel(const __grid_constant__ CUtensorMap map_k,
         if (n_tiles > 0) {
             constexpr uint32_t ID_S = tc_idesc(TA_TILE, false), ID_O = tc_idesc(PR_HD, true);
             const uint64_t desc_q = tc_desc(smem_u32(sm.q), 16, 1024),
-                           desc_k = tc_desc(smem_u32(sm.ring), 16, 1024),
-                           desc_v = tc_desc(smem_u32(sm.ring), TA_HALF, 1024);
+                           desc_k = tc_desc(smem_u32(sm.ring), 16, 2048),
+                           desc_v = tc_desc(smem_u32(sm.ring), 1024, 2048);
             int slot = 0, taken = 0;
             auto take = [&]() {                     // the next tile of the ring
                 const int s = slot;
@@ -296,8 +299,9 @@ tile_attn_kernel(const __grid_constant__ CUtensorMap map_k,
                 if (tc_elect()) {
 #pragma unroll
                     for (int ks = 0; ks < 8; ++ks) {
-                        const uint64_t off = (uint64_t)(((ks >> 2) * TA_HALF + (ks & 3) * 32) >> 4);
-                        tc_mma_ss(tmem + TM_S + i * TA_TILE, a + off, b + off, ID_S, ks ? 1u : 0u);
+                        const uint64_t in_row = (ks & 3) * 32 >> 4, half = ks >> 2;
+                        tc_mma_ss(tmem + TM_S + i * TA_TILE, a + in_row + half * (TA_HALF >> 4),
+                                  b + in_row + half * (1024 >> 4), ID_S, ks ? 1u : 0u);
                     }
                     tc_commit(&sm.s_full[i]);
                 }
@@ -599,18 +603,19 @@ tile_attn_kernel(const __grid_constant__ CUtensorMap map_k,
     }
 }
 
-// A cache plane as (128 channels, n_kv heads, 16 tokens, num_blocks) with its own
-// strides, boxes of 64 channels x 16 tokens of one head and block
+// A cache plane as (64 channels, 8 tokens, chunks of 64 channels, token groups of a
+// page, blocks): a head is two chunks, `sh / 64` chunks from the next head
 CUresult encode_plane(CUtensorMap* map, const void* base, int n_kv, int num_blocks,
                       int64_t sh, int64_t st, int64_t sb) {
     EncodeTiledFn enc = encode_tiled();
     if (enc == nullptr) return CUDA_ERROR_NOT_SUPPORTED;
-    const cuuint64_t dim[4] = {PR_HD, (cuuint64_t)n_kv, PR_PAGE, (cuuint64_t)num_blocks};
+    const int64_t chunks = (n_kv - 1) * (sh / 64) + 2;
+    const cuuint64_t dim[5] = {64, 8, (cuuint64_t)chunks, 2, (cuuint64_t)num_blocks};
     // (a dimension of one may come with any stride)
-    const cuuint64_t stride[3] = {(cuuint64_t)(n_kv > 1 ? sh : PR_HD) * 2, (cuuint64_t)st * 2,
+    const cuuint64_t stride[4] = {(cuuint64_t)st * 2, 128, (cuuint64_t)st * 16,
                                   (cuuint64_t)(num_blocks > 1 ? sb : PR_PAGE * st) * 2};
-    const cuuint32_t box[4] = {64, 1, PR_PAGE, 1}, one[4] = {1, 1, 1, 1};
-    return enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dim, stride,
+    const cuuint32_t box[5] = {64, 8, 2, 2, 1}, one[5] = {1, 1, 1, 1, 1};
+    return enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, const_cast<void*>(base), dim, stride,
                box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
 }
@@ -641,11 +646,13 @@ __global__ void __launch_bounds__(32 * TJ_WARPS) join_parts_kernel(const TileAtt
 
 }  // namespace
 
-int launch_tile_attn(const char* who, const TileAttnParams& p, int max_tiles, cudaStream_t s) {
+int launch_tile_attn(const char* who, TileAttnParams p, int max_tiles, cudaStream_t s) {
+    p.head_chunks = p.r.n_kv > 1 ? (int)(p.r.sh / 64) : 0;
     CUtensorMap mk, mv;
-    CUresult cr = encode_plane(&mk, p.r.k, p.r.n_kv, p.r.num_blocks, p.r.sh, p.r.st, p.r.sb);
+    CUresult cr = encode_plane(&mk, p.r.k, p.r.n_kv, p.r.num_blocks, 64 * p.head_chunks, p.r.st, p.r.sb);
     if (cr == CUDA_SUCCESS)
-        cr = encode_plane(&mv, p.r.v, p.r.n_kv, p.r.num_blocks, p.r.sh, p.r.st, p.r.sb);
+        cr = encode_plane(&mv, p.r.v, p.r.n_kv, p.r.num_blocks, 64 * p.head_chunks, p.r.st,
+                          p.r.sb);
     LOCKS_REQUIRE(cr == CUDA_SUCCESS, LOCKS_ERR_LAUNCH,
                   "%s: cuTensorMapEncodeTiled failed (%d)", who, (int)cr);
     static bool attr_done[64] = {false};
