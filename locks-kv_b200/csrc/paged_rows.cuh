@@ -123,6 +123,7 @@ struct TileAttnParams {
     float *parts_out, *parts_ml;
     int* status;
     int head_chunks;                  // 64-channel chunks between two heads
+    int max_tiles;                    // upper bound of the row tiles of all segments
 };
 
 // csrc/row_attn.cu; `who` names the entry point in error messages

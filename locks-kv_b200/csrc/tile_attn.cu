@@ -5,9 +5,9 @@
 // A "segment" is a run of query tokens that read one table row: a request's new
 // tokens, or the single tokens of the requests that share a prefix.  Its rows
 // (token, query head of the KV head) are packed, row = token * G + head, and cut
-// into tiles of up to 256.  One CTA takes a tile of one KV head and walks the pages
-// the tile can see -- first pages and recent ones as one list -- eight pages = 128
-// keys at a time:
+// into tiles of up to 256.  A work item is a tile of one KV head (and one part of its
+// keys); it walks the pages the tile can see -- first pages and recent ones as one
+// list -- eight pages = 128 keys at a time:
 //
 //   S [128 rows x 128 keys] = Q K^T       tcgen05.mma, Q and K in shared memory
 //   P = exp2(scale (S - m)), l += sum P   a thread per row: its row of S comes from
@@ -17,22 +17,24 @@
 // Two such streams run against each other, so that one's softmax hides behind the
 // other's products.  With more than 128 rows each stream has 128 of them and both
 // walk every key tile; with fewer, both have the same rows and take the key tiles in
-// turn (joined at the end through shared memory): a decode batch is then not half
-// idle.
+// turn (joined at the end: both O are in the same tensor-memory lanes): a decode batch
+// is then not half idle.
 //
+// One CTA per SM works through its share of the items; every stage runs ahead of the
+// next one across item borders, so that an item's start (finding it, Q, the first
+// pages: about 8 us when nothing overlaps it) and its end hide behind its neighbours.
 // Warps 0-3 and 4-7: softmax of stream 0 and 1 (thread = row = tensor-memory lane).
 // Warp 8: one thread issues all products.  Warp 9: fetches pages through the table by
-// tiled tensor-map copies (a page of a KV head is two boxes of 16 tokens x 64
-// channels, 128-byte swizzle) into a ring of five 32 KiB tiles that K and V share.
+// tiled tensor-map copies into a ring of four 32 KiB tiles that K and V share.
+// Warp 10: finds the items.  Warp 11: Q.
 // Tensor memory: S / P of the streams in columns 0 and 128, O in 256 and 384.
 //
-// The running maximum is only raised when it grows by more than 2^8 (O and l then
-// get rescaled): P stays below 2^8 and no row of O is touched in most steps.  P is
-// rounded to bf16 because V is (both operands of the product have one type), half a
-// step each; m, l, S and O are fp32.
+// The running maximum is only raised when it grows by more than 2^8 (O and l then get
+// rescaled): P stays below 2^8 and no row of O is touched in most steps.  P is rounded to bf16 because V is (both operands of the
+// product have one type), half a step each; m, l, S and O are fp32.
 //
-// Every wait is bounded (status word; later waits then return at once, copies in
-// flight are waited for and tensor memory is freed).  No multicast.
+// Every wait is bounded (status word; later waits then return at once, work and copies
+// in flight are waited for and tensor memory is freed).  No multicast.
 #include "common.cuh"
 #include "paged_rows.cuh"
 #include "tcgen05.cuh"
@@ -41,8 +43,8 @@
 namespace locks {
 namespace {
 
-constexpr int TA_THREADS = 320;
-constexpr int TA_RING = 5;
+constexpr int TA_THREADS = 384;
+constexpr int TA_RING = 4;
 constexpr int TA_TILE = 128;                       // keys of a tile, rows of a stream
 constexpr int TA_PAGES = TA_TILE / PR_PAGE;
 constexpr int TA_HALF = TA_TILE * 128;             // bytes: 128 rows x 64 channels
@@ -50,19 +52,29 @@ constexpr int TA_BYTES = 2 * TA_HALF;
 constexpr int TA_BOX = PR_PAGE * 256;              // bytes of a page of one plane and head
 constexpr int TM_S = 0, TM_O = 256, TM_COLS = 512;
 constexpr float TA_RAISE = 8.f;
+// P is handed over in two steps, so that the product of the first is under way while
+// the exponentials of the second are taken
+constexpr int TA_EARLY = 6;                        // pages (k-steps) of the first step
+
+struct Item {
+    int valid, seg, kh, part, t0, row0, n_rows, j0, n_tiles, key_end, written, base_pos;
+    int table_row;
+    PageList list;
+};
 
 struct __align__(1024) TileSmem {
     uint8_t q[2][TA_BYTES];
     uint8_t ring[TA_RING][TA_BYTES];
-    uint64_t full[TA_RING], empty[TA_RING], tail;
-    uint64_t q_full, s_full[2], p_ready[2], o_full[2];
+    uint8_t stage[8][4096];                        // a softmax warp's way out: 32 rows x 128 B
+    uint64_t full[TA_RING], empty[TA_RING], tail, drain;
+    uint64_t item_full[2], item_empty[2], q_full[2], q_empty;
+    uint64_t s_full[2], p_early[2], p_ready[2], o_full[2];
+    Item item[2];
     uint32_t tmem_base;
     int dead;
-    int scan[TA_THREADS / 32];
-    int seg, seg_tile, seg_tiles;
-    float xm[TA_TILE], xl[TA_TILE];
 };
 static_assert(sizeof(TileSmem) + 1024 <= 232448, "one CTA's shared memory");
+constexpr int TA_READERS = 11;                     // warps that read an item: all but its finder
 
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
@@ -87,18 +99,26 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
 }
 
 // a wait that gives up once any wait of the CTA has
+__device__ __forceinline__ bool is_dead(TileSmem& sm) {
+    return *reinterpret_cast<volatile int*>(&sm.dead) != 0;
+}
 __device__ __forceinline__ void ta_wait(TileSmem& sm, uint64_t* bar, uint32_t parity,
                                         int* status) {
-    if (mbar_try_wait(bar, parity)) return;
-    for (int it = 0; it < (1 << 22); ++it) {
-        if (mbar_try_wait(bar, parity)) return;
-        if (it > 64) {
-            __nanosleep(32);
-            if (*reinterpret_cast<volatile int*>(&sm.dead)) return;
+    if (!mbar_try_wait(bar, parity)) {
+        bool ok = false;
+        for (int it = 0; it < (1 << 22) && !ok; ++it) {
+            ok = mbar_try_wait(bar, parity);
+            if (!ok && it > 64) {
+                __nanosleep(32);
+                if (is_dead(sm)) break;
+            }
+        }
+        if (!ok && !is_dead(sm)) {
+            *reinterpret_cast<volatile int*>(&sm.dead) = 1;
+            if (status) atomicExch(status, LOCKS_ST_WAIT_TIMEOUT);
         }
     }
-    *reinterpret_cast<volatile int*>(&sm.dead) = 1;
-    if (status) atomicExch(status, LOCKS_ST_WAIT_TIMEOUT);
+    __syncwarp();
 }
 
 // 16 bytes global -> shared; src_bytes 0: zeros, nothing is read
@@ -127,15 +147,14 @@ __device__ __forceinline__ void segment(const TileAttnParams& p, int s, int& t0,
     n = max(n, 0);
 }
 
-// which segment tile `target` belongs to: a block-wide scan over the segments
-__device__ __forceinline__ bool find_tile(TileSmem& sm, const TileAttnParams& p, int target) {
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    if (tid == 0) sm.seg = -1;
+// Work item `w` (tile of a segment fastest, then KV head, then part), by one warp;
+// false: there is no such tile.
+__device__ __forceinline__ bool find_item(const TileAttnParams& p, int w, int lane, Item& it) {
+    const int target = w % p.max_tiles, rest = w / p.max_tiles;
     int before = 0;
-    for (int s0 = 0; s0 < p.n_seg; s0 += TA_THREADS) {
-        const int s = s0 + tid;
-        int t0, n = 0;
-        if (s < p.n_seg) segment(p, s, t0, n);
+    for (int s0 = 0; s0 < p.n_seg; s0 += 32) {
+        int t0 = 0, n = 0;
+        if (s0 + lane < p.n_seg) segment(p, s0 + lane, t0, n);
         const int mine = (n * p.r.G + 2 * TA_TILE - 1) / (2 * TA_TILE);
         int x = mine;
 #pragma unroll
@@ -143,24 +162,45 @@ __device__ __forceinline__ bool find_tile(TileSmem& sm, const TileAttnParams& p,
             const int y = __shfl_up_sync(0xffffffffu, x, d);
             if (lane >= d) x += y;
         }
-        __syncthreads();
-        if (lane == 31) sm.scan[warp] = x;
-        __syncthreads();
-        int mine_from = before + x - mine, total = before;
-#pragma unroll
-        for (int w = 0; w < TA_THREADS / 32; ++w) {
-            if (w < warp) mine_from += sm.scan[w];
-            total += sm.scan[w];
+        const int from = before + x - mine;
+        const uint32_t hit = __ballot_sync(0xffffffffu, target >= from && target < from + mine);
+        if (hit) {
+            const int src = __ffs(hit) - 1;
+            it.seg = s0 + src;
+            it.t0 = __shfl_sync(0xffffffffu, t0, src);
+            n = __shfl_sync(0xffffffffu, n, src);
+            // longest rows first
+            const int tile = __shfl_sync(0xffffffffu, mine - 1 - (target - from), src);
+            const int G = p.r.G;
+            it.kh = rest % p.r.n_kv;
+            it.part = rest / p.r.n_kv;
+            it.row0 = tile * 2 * TA_TILE;
+            it.n_rows = min(n * G - it.row0, 2 * TA_TILE);
+            it.base_pos = 0;
+            if (p.prefix_lens) {
+                const int whole = min(max(p.prefix_lens[it.seg], 0) / PR_PAGE, p.r.bt_width);
+                it.written = it.key_end = whole * PR_PAGE;
+                it.table_row = it.t0;
+                it.list = page_list(0, it.key_end - 1, INT32_MAX, 0, p.r.bt_width);
+            } else {
+                it.written = p.r.seq_lens[it.seg];
+                it.base_pos = it.written - n;
+                it.table_row = it.seg;
+                it.list = page_list(it.base_pos + it.row0 / G,
+                                    it.base_pos + (it.row0 + it.n_rows - 1) / G, p.r.window,
+                                    p.r.sinks, p.r.bt_width);
+                it.key_end = it.list.key_end;
+            }
+            const int all = (it.list.n + TA_PAGES - 1) / TA_PAGES;
+            const int per = (all + p.parts - 1) / p.parts;
+            it.j0 = min(it.part * per, all);
+            it.n_tiles = min(it.j0 + per, all) - it.j0;
+            it.valid = 1;
+            return true;
         }
-        if (target >= mine_from && target < mine_from + mine) {
-            sm.seg = s;
-            sm.seg_tile = mine - 1 - (target - mine_from);      // longest rows first
-        }
-        before = total;
-        if (before > target) break;
+        before += __shfl_sync(0xffffffffu, x, 31);
     }
-    __syncthreads();
-    return sm.seg >= 0;
+    return false;
 }
 
 __global__ void __launch_bounds__(TA_THREADS, 1)
@@ -169,45 +209,22 @@ tile_attn_kernel(const __grid_constant__ CUtensorMap map_k,
     extern __shared__ uint8_t ta_raw[];
     TileSmem& sm = *reinterpret_cast<TileSmem*>(
         ta_raw + ((1024u - (smem_u32(ta_raw) & 1023u)) & 1023u));
-    const int tid = threadIdx.x, lane = tid & 31;
+    const int tid = threadIdx.x, lane = tid & 31, G = p.r.G;
     const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);      // uniform, and known to be
-    const int kh = blockIdx.y, part = blockIdx.z, G = p.r.G;
-    if (!find_tile(sm, p, blockIdx.x)) return;
-    const int seg = sm.seg, row0 = sm.seg_tile * 2 * TA_TILE;
-    int t0, n_tok;
-    segment(p, seg, t0, n_tok);
-    const int rows = n_tok * G, n_rows = min(rows - row0, 2 * TA_TILE);
-    const bool by_rows = n_rows > TA_TILE;          // else both streams share the rows
-
-    // ---- keys of the tile --------------------------------------------------------
-    int key_end, written, base_pos = 0;             // written: keys behind it never were
-    const int32_t* table;
-    PageList list;
-    if (p.prefix_lens) {
-        const int whole = min(max(p.prefix_lens[seg], 0) / PR_PAGE, p.r.bt_width);
-        written = key_end = whole * PR_PAGE;
-        table = p.r.table + (int64_t)t0 * p.r.bt_stride;
-        list = page_list(0, key_end - 1, INT32_MAX, 0, p.r.bt_width);
-    } else {
-        written = p.r.seq_lens[seg];
-        base_pos = written - n_tok;
-        table = p.r.table + (int64_t)seg * p.r.bt_stride;
-        list = page_list(base_pos + row0 / G, base_pos + (row0 + n_rows - 1) / G,
-                         p.r.window, p.r.sinks, p.r.bt_width);
-        key_end = list.key_end;
-    }
-    const int all_tiles = (list.n + TA_PAGES - 1) / TA_PAGES;
-    const int per = (all_tiles + p.parts - 1) / p.parts;
-    const int j0 = min(part * per, all_tiles), n_tiles = min(j0 + per, all_tiles) - j0;
 
     // ---- setup -------------------------------------------------------------------
     if (tid == 0) {
         sm.dead = 0;
         for (int i = 0; i < TA_RING; ++i) { mbar_init(&sm.full[i], 1); mbar_init(&sm.empty[i], 1); }
         mbar_init(&sm.tail, 1);
-        mbar_init(&sm.q_full, 8);
+        mbar_init(&sm.drain, 1);
+        mbar_init(&sm.q_empty, 1);
         for (int i = 0; i < 2; ++i) {
+            mbar_init(&sm.item_full[i], 1);
+            mbar_init(&sm.item_empty[i], TA_READERS);
+            mbar_init(&sm.q_full[i], 1);
             mbar_init(&sm.s_full[i], 1);
+            mbar_init(&sm.p_early[i], 4);
             mbar_init(&sm.p_ready[i], 4);
             mbar_init(&sm.o_full[i], 1);
         }
@@ -223,203 +240,330 @@ tile_attn_kernel(const __grid_constant__ CUtensorMap map_k,
     tc_after_sync();
     const uint32_t tmem = sm.tmem_base;
 
-    if (warp == 9) {
-        // ---- pages: K and V tiles in the order the products take them ---------------
-        int slot = 0, issued = 0;
-        auto fetch = [&](int j, bool is_v) {
-            if (issued >= TA_RING)
-                ta_wait(sm, &sm.empty[slot], (uint32_t)((issued / TA_RING) - 1) & 1u, p.status);
-            if (__any_sync(0xffffffffu, *reinterpret_cast<volatile int*>(&sm.dead))) return;
-            const int v = (j0 + j) * TA_PAGES + (lane & 7);
-            int blk = p.r.num_blocks;               // outside the map: zeros
-            bool partial = false;
-            int page = 0;
-            if (v < list.n) {
-                page = list.page(v);
-                blk = min(max(table[page], 0), p.r.num_blocks - 1);
-                partial = is_v && (page + 1) * PR_PAGE > written;
-            }
-            const uint32_t cut = __ballot_sync(0xffffffffu, lane < 8 && partial);
-            uint64_t* bar = cut ? &sm.tail : &sm.full[slot];
-            if (lane == 0) mbar_expect_tx(bar, TA_BYTES);
-            __syncwarp();
-            if (lane < TA_PAGES)
-                tma_load_page(&sm.ring[slot][lane * TA_BOX], is_v ? &map_v : &map_k,
-                              kh * p.head_chunks, blk, bar);
-            if (cut) {
-                // the sequence ends inside a page: what the cache holds behind it may
-                // be anything, and 0 x NaN is not 0
-                ta_wait(sm, &sm.tail, 0, p.status);
+    // the n-th item of this CTA: null when there is none (or a wait ran out)
+    auto next_item = [&](int n) -> const Item* {
+        ta_wait(sm, &sm.item_full[n & 1], (uint32_t)(n >> 1) & 1u, p.status);
+        if (__any_sync(0xffffffffu, is_dead(sm))) return nullptr;
+        return sm.item[n & 1].valid ? &sm.item[n & 1] : nullptr;
+    };
+    auto done_with = [&](int n) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.item_empty[n & 1]);
+    };
+
+    // registers: 12 warps start with 168 each; the softmax threads hold a row of S
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        if (warp == 10) {
+            // ---- items ----------------------------------------------------------------
+            const int total = p.max_tiles * p.r.n_kv * p.parts;
+            int n = 0;
+            for (int w = blockIdx.x; !__any_sync(0xffffffffu, is_dead(sm)); w += gridDim.x) {
+                Item it;
+                it.valid = 0;
+                if (w < total && !find_item(p, w, lane, it)) continue;
+                if (n >= 2)
+                    ta_wait(sm, &sm.item_empty[n & 1], (uint32_t)((n >> 1) - 1) & 1u, p.status);
+                if (lane == 0) {
+                    sm.item[n & 1] = it;
+                    mbar_arrive(&sm.item_full[n & 1]);
+                }
                 __syncwarp();
-                const int s = __ffs(cut) - 1;
-                const int from = max(written - __shfl_sync(0xffffffffu, page, s) * PR_PAGE, 0);
-                for (int e = lane; e < (PR_PAGE - from) * 16; e += 32)
-                    *reinterpret_cast<uint4*>(
-                        &sm.ring[slot][s * TA_BOX + ((from + (e >> 4)) >> 3) * 2048 +
-                                       ((e >> 3) & 1) * 1024 + ((from + (e >> 4)) & 7) * 128 +
-                                       (e & 7) * 16]) = make_uint4(0, 0, 0, 0);
-                fence_proxy_async();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&sm.full[slot]);
+                ++n;
+                if (!it.valid) break;
             }
-            slot = slot + 1 == TA_RING ? 0 : slot + 1;
-            ++issued;
-        };
-        if (n_tiles > 0) fetch(0, false);
-        if (!by_rows && n_tiles > 1) fetch(1, false);
-        for (int j = 0; j < n_tiles; ++j) {
-            fetch(j, true);
-            const int next = by_rows ? j + 1 : j + 2;
-            if (next < n_tiles) fetch(next, false);
-        }
-        // a wait ran out: nobody consumed the last copies; they must land all the same
-        if (*reinterpret_cast<volatile int*>(&sm.dead))
-            for (int i = max(issued - TA_RING, 0); i < issued; ++i)
-                mbar_wait(&sm.full[i % TA_RING], (uint32_t)(i / TA_RING) & 1u, p.status);
-    } else if (warp == 8) {
-        // ---- products -------------------------------------------------------------
-        if (n_tiles > 0) {
+        } else if (warp == 11) {
+            // ---- Q into the swizzled K-major layout, 16 lanes to a row -------------------
+            int loads = 0;
+            for (int n = 0;; ++n) {
+                const Item* item = next_item(n);
+                if (!item) break;
+                const int row0 = item->row0, n_rows = item->n_rows, t0 = item->t0,
+                          kh = item->kh, n_tiles = item->n_tiles;
+                done_with(n);
+                if (n_tiles == 0) continue;
+                if (loads > 0)
+                    ta_wait(sm, &sm.q_empty, (uint32_t)(loads - 1) & 1u, p.status);
+                ++loads;
+                // (rows behind the last one are zeros; every copy is on its way before
+                // the first is waited for)
+                const int piece = lane & 15;
+                int row = lane >> 4, tok = (row0 + row) / G, g = row0 + row - tok * G;
+                const __nv_bfloat16* src = p.r.q + (int64_t)(t0 + tok) * p.r.q_tok +
+                                           (int64_t)(kh * G + g) * p.r.q_head + 8 * piece;
+                // two rows on: in the same token, or in the next one (G = 1: the one after)
+                const int64_t stay = 2 * p.r.q_head,
+                              wrap = G == 1 ? 2 * p.r.q_tok : p.r.q_tok + (2 - G) * p.r.q_head;
+                const uint32_t d0 = smem_u32(sm.q) + (piece >> 3) * TA_HALF;
+                for (int sub = 0; sub < (n_rows > TA_TILE ? 2 : 1); ++sub) {
+#pragma unroll 8
+                    for (int k = 0; k < TA_TILE / 2; ++k) {
+                        const bool live = row < n_rows;
+                        const int r = row & (TA_TILE - 1);
+                        cp_async16(d0 + sub * TA_BYTES + r * 128 + ((piece ^ r) & 7) * 16,
+                                   live ? src : p.r.q, live ? 16 : 0);
+                        const bool over = g + 2 >= G;
+                        src += over ? wrap : stay;
+                        g = G == 1 ? 0 : g + 2 - (over ? G : 0);
+                        row += 2;
+                    }
+                    asm volatile("cp.async.wait_all;" ::: "memory");
+                    fence_proxy_async();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sm.q_full[sub]);
+                }
+            }
+        } else if (warp == 9) {
+            // ---- pages: K and V tiles in the order the products take them ---------------
+            int slot = 0, issued = 0, cuts = 0;
+            for (int n = 0;; ++n) {
+                const Item* item = next_item(n);
+                if (!item) break;
+                const PageList list = item->list;
+                const int j0 = item->j0, n_tiles = item->n_tiles, written = item->written;
+                const int chunk = item->kh * p.head_chunks;
+                const bool by_rows = item->n_rows > TA_TILE;
+                const int32_t* table = p.r.table + (int64_t)item->table_row * p.r.bt_stride;
+                done_with(n);
+                auto fetch = [&](int j, bool is_v) {
+                    const int v = (j0 + j) * TA_PAGES + (lane & 7);
+                    int blk = p.r.num_blocks;           // outside the map: zeros
+                    bool partial = false;
+                    int page = 0;
+                    if (v < list.n) {
+                        page = list.page(v);
+                        blk = min(max(table[page], 0), p.r.num_blocks - 1);
+                        partial = is_v && (page + 1) * PR_PAGE > written;
+                    }
+                    if (issued >= TA_RING)
+                        ta_wait(sm, &sm.empty[slot], (uint32_t)((issued / TA_RING) - 1) & 1u,
+                                p.status);
+                    if (__any_sync(0xffffffffu, is_dead(sm))) return;
+                    const uint32_t cut = __ballot_sync(0xffffffffu, lane < 8 && partial);
+                    uint64_t* bar = cut ? &sm.tail : &sm.full[slot];
+                    if (lane == 0) mbar_expect_tx(bar, TA_BYTES);
+                    __syncwarp();
+                    if (lane < TA_PAGES)
+                        tma_load_page(&sm.ring[slot][lane * TA_BOX], is_v ? &map_v : &map_k,
+                                      chunk, blk, bar);
+                    if (cut) {
+                        // the sequence ends inside a page: what the cache holds behind it
+                        // may be anything, and 0 x NaN is not 0
+                        ta_wait(sm, &sm.tail, (uint32_t)cuts & 1u, p.status);
+                        ++cuts;
+                        const int s = __ffs(cut) - 1;
+                        const int from =
+                            max(written - __shfl_sync(0xffffffffu, page, s) * PR_PAGE, 0);
+                        for (int e = lane; e < (PR_PAGE - from) * 16; e += 32)
+                            *reinterpret_cast<uint4*>(
+                                &sm.ring[slot][s * TA_BOX + ((from + (e >> 4)) >> 3) * 2048 +
+                                               ((e >> 3) & 1) * 1024 +
+                                               ((from + (e >> 4)) & 7) * 128 + (e & 7) * 16]) =
+                                make_uint4(0, 0, 0, 0);
+                        fence_proxy_async();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&sm.full[slot]);
+                    }
+                    slot = slot + 1 == TA_RING ? 0 : slot + 1;
+                    ++issued;
+                };
+                if (n_tiles > 0) fetch(0, false);
+                if (!by_rows && n_tiles > 1) fetch(1, false);
+                for (int j = 0; j < n_tiles; ++j) {
+                    fetch(j, true);
+                    const int next = by_rows ? j + 1 : j + 2;
+                    if (next < n_tiles) fetch(next, false);
+                }
+            }
+            // a wait ran out: nobody consumed the last copies; they must land all the same
+            if (__any_sync(0xffffffffu, is_dead(sm)))
+                for (int i = max(issued - TA_RING, 0); i < issued; ++i)
+                    mbar_wait(&sm.full[i % TA_RING], (uint32_t)(i / TA_RING) & 1u, p.status);
+        } else if (warp == 8) {
+            // ---- products -------------------------------------------------------------
             constexpr uint32_t ID_S = tc_idesc(TA_TILE, false), ID_O = tc_idesc(PR_HD, true);
             const uint64_t desc_q = tc_desc(smem_u32(sm.q), 16, 1024),
                            desc_k = tc_desc(smem_u32(sm.ring), 16, 2048),
                            desc_v = tc_desc(smem_u32(sm.ring), 1024, 2048);
-            int slot = 0, taken = 0;
+            int slot = 0, taken = 0, loads = 0, both = 0;
+            uint32_t phase[2] = {0, 0};             // tiles of each stream, over all items
             auto take = [&]() {                     // the next tile of the ring
                 const int s = slot;
                 ta_wait(sm, &sm.full[s], (uint32_t)(taken / TA_RING) & 1u, p.status);
-                __syncwarp();
                 slot = slot + 1 == TA_RING ? 0 : slot + 1;
                 ++taken;
                 return s;
             };
-            auto scores = [&](int i, int s) {
-                tc_after_sync();
-                const uint64_t a = desc_q + (uint64_t)((by_rows ? i : 0) * (TA_BYTES >> 4));
-                const uint64_t b = desc_k + (uint64_t)(s * (TA_BYTES >> 4));
-                if (tc_elect()) {
+            auto commit = [&](uint64_t* bar) {
+                if (tc_elect()) tc_commit(bar);
+                __syncwarp();
+            };
+            for (int n = 0;; ++n) {
+                const Item* item = next_item(n);
+                if (!item) break;
+                const int n_tiles = item->n_tiles;
+                const bool by_rows = item->n_rows > TA_TILE;
+                done_with(n);
+                if (n_tiles == 0) continue;
+                auto scores = [&](int i, int s) {
+                    tc_after_sync();
+                    const uint64_t a = desc_q + (uint64_t)((by_rows ? i : 0) * (TA_BYTES >> 4));
+                    const uint64_t b = desc_k + (uint64_t)(s * (TA_BYTES >> 4));
+                    if (tc_elect()) {
 #pragma unroll
-                    for (int ks = 0; ks < 8; ++ks) {
-                        const uint64_t in_row = (ks & 3) * 32 >> 4, half = ks >> 2;
-                        tc_mma_ss(tmem + TM_S + i * TA_TILE, a + in_row + half * (TA_HALF >> 4),
-                                  b + in_row + half * (1024 >> 4), ID_S, ks ? 1u : 0u);
+                        for (int ks = 0; ks < 8; ++ks) {
+                            const uint64_t in_row = (ks & 3) * 32 >> 4, half = ks >> 2;
+                            tc_mma_ss(tmem + TM_S + i * TA_TILE,
+                                      a + in_row + half * (TA_HALF >> 4),
+                                      b + in_row + half * (1024 >> 4), ID_S, ks ? 1u : 0u);
+                        }
+                        tc_commit(&sm.s_full[i]);
                     }
-                    tc_commit(&sm.s_full[i]);
-                }
-                __syncwarp();
-            };
-            auto values = [&](int i, int s, int t) { // stream i's tile number t
-                ta_wait(sm, &sm.p_ready[i], (uint32_t)t & 1u, p.status);
-                __syncwarp();
-                tc_after_sync();
-                const uint64_t b = desc_v + (uint64_t)(s * (TA_BYTES >> 4));
-                if (tc_elect()) {
+                    __syncwarp();
+                };
+                auto values = [&](int i, int s, int t) {    // the item's tile t of stream i
+                    const uint64_t b = desc_v + (uint64_t)(s * (TA_BYTES >> 4));
+                    const uint32_t par = phase[i]++ & 1u;
 #pragma unroll
-                    for (int ks = 0; ks < TA_PAGES; ++ks)
-                        tc_mma_ts(tmem + TM_O + i * PR_HD, tmem + TM_S + i * TA_TILE + ks * 8,
-                                  b + (uint64_t)((ks * TA_BOX) >> 4), ID_O, (t | ks) ? 1u : 0u);
-                    tc_commit(&sm.o_full[i]);
-                }
-                __syncwarp();
-            };
-            auto release = [&](int s) {
-                if (tc_elect()) tc_commit(&sm.empty[s]);
-                __syncwarp();
-            };
-            int k_slot = take();
-            ta_wait(sm, &sm.q_full, 0, p.status);
-            __syncwarp();
-            scores(0, k_slot);
-            if (by_rows) {
-                scores(1, k_slot);
-                release(k_slot);
-                for (int j = 0; j < n_tiles; ++j) {
-                    const int v_slot = take();
-                    values(0, v_slot, j);
-                    if (j + 1 < n_tiles) {
-                        k_slot = take();
-                        scores(0, k_slot);
+                    for (int half = 0; half < 2; ++half) {
+                        ta_wait(sm, half ? &sm.p_ready[i] : &sm.p_early[i], par, p.status);
+                        tc_after_sync();
+                        if (tc_elect()) {
+#pragma unroll
+                            for (int ks = half ? TA_EARLY : 0; ks < (half ? TA_PAGES : TA_EARLY);
+                                 ++ks)
+                                tc_mma_ts(tmem + TM_O + i * PR_HD, tmem + TM_S + i * TA_TILE + ks * 8,
+                                          b + (uint64_t)((ks * TA_BOX) >> 4), ID_O,
+                                          (t | ks) ? 1u : 0u);
+                            if (half) tc_commit(&sm.o_full[i]);
+                        }
+                        __syncwarp();
                     }
-                    values(1, v_slot, j);
-                    release(v_slot);
-                    if (j + 1 < n_tiles) {
-                        scores(1, k_slot);
-                        release(k_slot);
-                    }
-                }
-            } else {
-                release(k_slot);
-                if (n_tiles > 1) {
-                    k_slot = take();
+                };
+                int k_slot = take();
+                ta_wait(sm, &sm.q_full[0], (uint32_t)loads & 1u, p.status);
+                ++loads;
+                scores(0, k_slot);
+                if (by_rows) {
+                    ta_wait(sm, &sm.q_full[1], (uint32_t)both & 1u, p.status);
+                    ++both;
                     scores(1, k_slot);
-                    release(k_slot);
-                }
-                for (int j = 0; j < n_tiles; ++j) {
-                    const int v_slot = take();
-                    values(j & 1, v_slot, j >> 1);
-                    release(v_slot);
-                    if (j + 2 < n_tiles) {
+                    commit(&sm.empty[k_slot]);
+                    if (n_tiles == 1) commit(&sm.q_empty);
+                    // (the ring's next tiles are waited for while products run)
+                    int v_slot = take();
+                    for (int j = 0; j < n_tiles; ++j) {
+                        const bool more = j + 1 < n_tiles;
+                        if (more) k_slot = take();
+                        values(0, v_slot, j);
+                        if (more) scores(0, k_slot);
+                        values(1, v_slot, j);
+                        commit(&sm.empty[v_slot]);
+                        if (more) {
+                            scores(1, k_slot);
+                            commit(&sm.empty[k_slot]);
+                            if (j + 2 == n_tiles) commit(&sm.q_empty);
+                            v_slot = take();
+                        }
+                    }
+                } else {
+                    commit(&sm.empty[k_slot]);
+                    if (n_tiles > 1) {
                         k_slot = take();
-                        scores(j & 1, k_slot);
-                        release(k_slot);
+                        scores(1, k_slot);
+                        commit(&sm.empty[k_slot]);
+                    }
+                    if (n_tiles <= 2) commit(&sm.q_empty);
+                    for (int j = 0; j < n_tiles; ++j) {
+                        const int v_slot = take();
+                        values(j & 1, v_slot, j >> 1);
+                        commit(&sm.empty[v_slot]);
+                        if (j + 2 < n_tiles) {
+                            k_slot = take();
+                            scores(j & 1, k_slot);
+                            commit(&sm.empty[k_slot]);
+                            if (j + 3 == n_tiles) commit(&sm.q_empty);
+                        }
                     }
                 }
             }
-        }
-    } else if (warp < 8) {
-        // ---- Q into the swizzled K-major layout, 16 lanes to a row -------------------
-        {
-            // (rows behind the last one are zeros; every copy is on its way before the
-            // first is waited for)
-            const int piece = tid & 15;
-#pragma unroll 8
-            for (int k = 0; k < (by_rows ? 16 : 8); ++k) {
-                const int row = (tid >> 4) + 16 * k, at = row0 + min(row, n_rows - 1);
-                const int tok = at / G;
-                const __nv_bfloat16* src = p.r.q + (int64_t)(t0 + tok) * p.r.q_tok +
-                                           (int64_t)(kh * G + at - tok * G) * p.r.q_head +
-                                           8 * piece;
-                cp_async16(smem_u32(&sm.q[row >> 7][(piece >> 3) * TA_HALF +
-                                                    tc_swz(row & 127, (piece & 7) << 4)]),
-                           src, row < n_rows ? 16 : 0);
+            if (__any_sync(0xffffffffu, is_dead(sm))) {     // products in flight end first
+                commit(&sm.drain);
+                mbar_wait(&sm.drain, 0, p.status);
             }
-            asm volatile("cp.async.wait_all;" ::: "memory");
-            fence_proxy_async();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sm.q_full);
         }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
         // ---- softmax: stream i, thread = row ---------------------------------------
         const int i = warp >> 2, q4 = warp & 3;
-        const int local = (by_rows ? i * TA_TILE : 0) + q4 * 32 + lane;
-        const int row = row0 + min(local, n_rows - 1);
-        const int tok = row / G;
-        const int pos = p.prefix_lens ? p.r.seq_lens[t0 + tok] - 1 : base_pos + tok;
-        const int last_key = min(pos, key_end - 1);
-        const int first_key = pos >= p.r.window ? pos - p.r.window + 1 : 0;
-        const int sinks = p.r.sinks;
-        // (row order is position order only for a request's own tokens)
-        const int w_last = __reduce_min_sync(0xffffffffu, last_key);
-        const int w_first = __reduce_max_sync(0xffffffffu, first_key);
         const uint32_t lane_base = tmem + ((uint32_t)(q4 * 32) << 16);
-        const uint32_t ts = lane_base + TM_S + i * TA_TILE, to = lane_base + TM_O + i * PR_HD;
+        const uint32_t ts = lane_base + TM_S + i * TA_TILE;
         const float sl2 = p.r.scale_log2;
-        float m = -INFINITY, l = 0.f;
-        int t = 0;                                  // tiles of this stream so far
-        for (int j = by_rows ? 0 : i; j < n_tiles; j += by_rows ? 1 : 2, ++t) {
-            ta_wait(sm, &sm.s_full[i], (uint32_t)t & 1u, p.status);
-            __syncwarp();
-            tc_after_sync();
-            uint32_t sr[TA_TILE];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) tc_ld32(ts + 32 * c, sr + 32 * c);
-            tc_wait_ld();
-            float* s = reinterpret_cast<float*>(sr);
-            const int v0 = (j0 + j) * TA_PAGES;
+        uint32_t phase = 0;                         // tiles of this stream, over all items
+        for (int n = 0;; ++n) {
+            const Item* item = next_item(n);
+            if (!item) break;
+            const PageList list = item->list;
+            const int j0 = item->j0, n_tiles = item->n_tiles, n_rows = item->n_rows;
+            const bool by_rows = n_rows > TA_TILE;
+            const int local = (by_rows ? i * TA_TILE : 0) + q4 * 32 + lane;
+            const int row = item->row0 + min(local, n_rows - 1);
+            const int t0 = item->t0, tok = row / G, head = item->kh * G + row - tok * G;
+            const int pos = p.prefix_lens ? p.r.seq_lens[t0 + tok] - 1 : item->base_pos + tok;
+            const int last_key = min(pos, item->key_end - 1), part = item->part;
+            done_with(n);
+            const int first_key = pos >= p.r.window ? pos - p.r.window + 1 : 0;
+            const int sinks = p.r.sinks;
+            // (row order is position order only for a request's own tokens)
+            const int w_last = __reduce_min_sync(0xffffffffu, last_key);
+            const int w_first = __reduce_max_sync(0xffffffffu, first_key);
+            // tiles [clear_lo, clear_hi) hide no key from any row of the warp: keys up to
+            // the oldest row's, and either all first keys or all in the newest's window
+            int clear_lo, clear_hi;
             {
-                const int lo_key = list.page(v0) * PR_PAGE;
-                const int hi_key = list.page(v0 + TA_PAGES - 1) * PR_PAGE + PR_PAGE - 1;
-                const bool clear = v0 + TA_PAGES <= list.n && hi_key <= w_last &&
-                                   (lo_key >= w_first || hi_key < sinks);
-                if (!clear) {
+                const int n_win = max(w_last + 1, 0) / PR_PAGE - list.shift;    // entries before it
+                clear_hi = min(list.n, n_win) / TA_PAGES;
+                const int sink_hi = min(min(list.n_first, sinks / PR_PAGE),
+                                        max(w_last + 1, 0) / PR_PAGE) / TA_PAGES;
+                const int from = max((w_first + PR_PAGE - 1) / PR_PAGE - list.shift,
+                                     list.shift > 0 && w_first > 0 ? list.n_first : 0);
+                clear_lo = (from + TA_PAGES - 1) / TA_PAGES;
+                if (clear_hi <= clear_lo) { clear_lo = 0; clear_hi = sink_hi; }
+            }
+            float m = -INFINITY, l = 0.f;
+            int t = 0;                              // this item's tiles of this stream so far
+            for (int j = by_rows ? 0 : i; j < n_tiles; j += by_rows ? 1 : 2, ++t, ++phase) {
+                ta_wait(sm, &sm.s_full[i], phase & 1u, p.status);
+                tc_after_sync();
+                uint32_t sr[TA_TILE];
+                float* s = reinterpret_cast<float*>(sr);
+                float mx[8];
+                auto peaks = [&](int c0) {          // maxima of columns c0 .. c0 + 63
+#pragma unroll
+                    for (int c = c0; c < c0 + 64; c += 16)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            mx[e] = c == 0 ? fmaxf(s[e], s[8 + e]) : max3(mx[e], s[c + e], s[c + 8 + e]);
+                };
+                tc_ld32(ts, sr);
+                tc_ld32(ts + 32, sr + 32);
+                tc_wait_ld();
+                tc_tie32(sr);
+                tc_tie32(sr + 32);
+                tc_ld32(ts + 64, sr + 64);
+                tc_ld32(ts + 96, sr + 96);
+                const int jt = j0 + j;
+                if (jt >= clear_lo && jt < clear_hi) {
+                    peaks(0);
+                    tc_wait_ld();
+                    tc_tie32(sr + 64);
+                    tc_tie32(sr + 96);
+                    peaks(64);
+                } else {
+                    tc_wait_ld();
+                    tc_tie32(sr + 64);
+                    tc_tie32(sr + 96);
+                    const int v0 = jt * TA_PAGES;
 #pragma unroll
                     for (int pg = 0; pg < TA_PAGES; ++pg) {
                         uint32_t keep = 0;
@@ -436,163 +580,165 @@ tile_attn_kernel(const __grid_constant__ CUtensorMap map_k,
                         for (int c = 0; c < PR_PAGE; ++c)
                             if (!(keep >> c & 1u)) s[pg * PR_PAGE + c] = -INFINITY;
                     }
+                    peaks(0);
+                    peaks(64);
                 }
-            }
-            float mx[4] = {s[0], s[1], s[2], s[3]};
+                const float tile_max = max3(max3(mx[0], mx[1], mx[2]), max3(mx[3], mx[4], mx[5]),
+                                            fmaxf(mx[6], mx[7]));
+                if (t == 0) {
+                    m = tile_max;
+                } else if (__any_sync(0xffffffffu, (tile_max - m) * sl2 > TA_RAISE)) {
+                    // (m -inf: nothing seen so far, O and l are 0 and stay it)
+                    const float up = fmaxf(m, tile_max);
+                    const float f = m == -INFINITY ? 0.f : pr_exp2((m - up) * sl2);
+                    m = up;
+                    l *= f;
+                    ta_wait(sm, &sm.o_full[i], (phase - 1) & 1u, p.status);
+                    tc_after_sync();
+                    const uint32_t to = lane_base + TM_O + i * PR_HD;
 #pragma unroll
-            for (int c = 4; c < TA_TILE - 4; c += 8)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], s[c + e], s[c + 4 + e]);
-            const float tile_max =
-                fmaxf(max3(max3(mx[0], mx[1], mx[2]), mx[3], s[TA_TILE - 4]),
-                      max3(s[TA_TILE - 3], s[TA_TILE - 2], s[TA_TILE - 1]));
-            if (t == 0) {
-                m = tile_max;
-            } else if (__any_sync(0xffffffffu, (tile_max - m) * sl2 > TA_RAISE)) {
-                // (m -inf: nothing seen so far, O and l are 0 and stay it)
-                const float up = fmaxf(m, tile_max);
-                const float f = m == -INFINITY ? 0.f : pr_exp2((m - up) * sl2);
-                m = up;
-                l *= f;
-                ta_wait(sm, &sm.o_full[i], (uint32_t)(t - 1) & 1u, p.status);
-                __syncwarp();
-                tc_after_sync();
-#pragma unroll
-                for (int c = 0; c < 8; ++c) {
-                    uint32_t o[16];
-                    tc_ld16(to + 16 * c, o);
-                    tc_wait_ld();
-#pragma unroll
-                    for (int e = 0; e < 16; ++e)
-                        o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                    tc_st16(to + 16 * c, o);
-                }
-            }
-            const float base = m == -INFINITY ? 0.f : m * sl2;
-            const float2 k2 = make_float2(sl2, sl2), b2 = make_float2(-base, -base);
-            float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                uint32_t pk[16];
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    float2 x = fma2(make_float2(s[32 * c + 2 * e], s[32 * c + 2 * e + 1]), k2, b2);
-                    x.x = pr_exp2(x.x);
-                    x.y = pr_exp2(x.y);
-                    sum[e & 1] = add2(sum[e & 1], x);
-                    pk[e] = pack_bf16x2(x.x, x.y);
-                }
-                tc_st16(ts + 16 * c, pk);
-            }
-            l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
-            tc_wait_st();
-            tc_before_sync();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sm.p_ready[i]);
-        }
-        // ---- results ---------------------------------------------------------------
-        if (t > 0) {
-            ta_wait(sm, &sm.o_full[i], (uint32_t)(t - 1) & 1u, p.status);
-            __syncwarp();
-            tc_after_sync();
-        }
-        // streams that share the rows: stream 1 hands over (m, l, O), column by column
-        // (lane = bank), stream 0 weighs both
-        float w0 = 1.f, w1 = 0.f;
-        float* xo = reinterpret_cast<float*>(sm.ring[0]);
-        if (!by_rows) {
-            const int at = q4 * 32 + lane;
-            // (both streams' last products are done: the ring is idle)
-            asm volatile("bar.sync 1, 256;" ::: "memory");
-            if (i == 1) {
-                sm.xm[at] = m;
-                sm.xl[at] = l;
-                if (t > 0)
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        uint32_t o[32];
-                        tc_ld32(to + 32 * c, o);
+                    for (int c = 0; c < 8; ++c) {
+                        uint32_t o[16];
+                        tc_ld16(to + 16 * c, o);
                         tc_wait_ld();
+                        tc_tie16(o);
 #pragma unroll
-                        for (int e = 0; e < 32; ++e)
-                            xo[(32 * c + e) * TA_TILE + at] = __uint_as_float(o[e]);
+                        for (int e = 0; e < 16; ++e)
+                            o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                        tc_st16(to + 16 * c, o);
                     }
-            }
-            asm volatile("bar.sync 1, 256;" ::: "memory");
-            if (i == 0) {
-                const float m1 = sm.xm[at], l1 = sm.xl[at];
-                const float up = fmaxf(m, m1);
-                w0 = l > 0.f ? pr_exp2((m - up) * sl2) : 0.f;
-                w1 = l1 > 0.f ? pr_exp2((m1 - up) * sl2) : 0.f;
-                l = w0 * l + w1 * l1;
-                m = up;
-            }
-        }
-        if ((by_rows || i == 0) && p.parts_out == nullptr) {
-            const float inv = l > 0.f ? 1.f / l : 0.f;
-            const int h = kh * G + row - tok * G;
-            __nv_bfloat16* out = p.r.out + (int64_t)(t0 + tok) * p.r.o_tok + (int64_t)h * p.r.o_head;
-            const bool second = w1 > 0.f;
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                uint32_t o[32];
-                if (t > 0) {
-                    tc_ld32(to + 32 * c, o);
-                    tc_wait_ld();
                 }
-#pragma unroll
-                for (int e = 0; e < 32; e += 8) {
-                    float f[8];
-#pragma unroll
-                    for (int x = 0; x < 8; ++x) {
-                        f[x] = l > 0.f && w0 > 0.f ? w0 * __uint_as_float(o[e + x]) : 0.f;
-                        if (second)
-                            f[x] += w1 * xo[(32 * c + e + x) * TA_TILE + q4 * 32 + lane];
-                        f[x] *= inv;
-                    }
-                    if (local < n_rows)
-                        *reinterpret_cast<uint4*>(out + 32 * c + e) =
-                            make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]),
-                                       pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
-                }
-            }
-            if (p.r.lse && local < n_rows)
-                p.r.lse[(int64_t)(t0 + tok) * p.r.lse_tok + h] =
-                    l > 0.f ? (m * sl2 + log2f(l)) * PR_LN2 : -INFINITY;
-        } else if (by_rows || i == 0) {
-            // one of several parts: O relative to m, with (m in log2 units, l)
-            const int h = kh * G + row - tok * G;
-            const int64_t at = (int64_t)part * p.part_rows + (int64_t)(t0 + tok) * p.r.n_kv * G + h;
-            float* out = p.parts_out + at * PR_HD;
-            const bool second = w1 > 0.f;
-            if (__any_sync(0xffffffffu, l > 0.f)) {
+                const float base = m == -INFINITY ? 0.f : m * sl2;
+                const float2 k2 = make_float2(sl2, sl2), b2 = make_float2(-base, -base);
+                float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
-                    uint32_t o[32];
-                    if (t > 0) {
-                        tc_ld32(to + 32 * c, o);
-                        tc_wait_ld();
+                    uint32_t pk[16];
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        float2 x = fma2(make_float2(s[32 * c + 2 * e], s[32 * c + 2 * e + 1]), k2, b2);
+                        x.x = pr_exp2(x.x);
+                        x.y = pr_exp2(x.y);
+                        sum[e & 1] = add2(sum[e & 1], x);
+                        pk[e] = pack_bf16x2(x.x, x.y);
                     }
+                    tc_st16(ts + 16 * c, pk);
+                    if (2 * (c + 1) == TA_EARLY || c == 3) {
+                        tc_wait_st();
+                        tc_before_sync();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(c == 3 ? &sm.p_ready[i] : &sm.p_early[i]);
+                    }
+                }
+                l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+            }
+            // ---- results: columns [from, from + 32 chunks) of O ---------------------------
+            if (t > 0) {
+                ta_wait(sm, &sm.o_full[i], (phase - 1) & 1u, p.status);
+                tc_after_sync();
+            }
+            // streams that share the rows: each finishes half of the channels
+            const int chunk0 = by_rows ? 0 : 2 * i, chunks = by_rows ? 4 : 2;
+            float w_mine = l > 0.f ? 1.f : 0.f, w_other = 0.f;
+            if (!by_rows) {
+                float2* mine = reinterpret_cast<float2*>(sm.stage[warp]) + lane;
+                *mine = make_float2(m, l);
+                tc_before_sync();
+                asm volatile("bar.sync 1, 256;" ::: "memory");
+                tc_after_sync();
+                const float2 other = reinterpret_cast<float2*>(sm.stage[warp ^ 4])[lane];
+                asm volatile("bar.sync 1, 256;" ::: "memory");
+                const float m1 = other.x, l1 = other.y;
+                const float up = fmaxf(m, m1);
+                w_mine = l > 0.f ? pr_exp2((m - up) * sl2) : 0.f;
+                w_other = l1 > 0.f ? pr_exp2((m1 - up) * sl2) : 0.f;
+                l = w_mine * l + w_other * l1;
+                m = up;
+            }
+            const bool final = p.parts_out == nullptr;
+            const float inv = !final ? 1.f : l > 0.f ? 1.f / l : 0.f;
+            w_mine *= inv;
+            w_other *= inv;
+            const int64_t part_at = (int64_t)part * p.part_rows +
+                                    (int64_t)(t0 + tok) * p.r.n_kv * G + head;
+            // a row's way out: through the warp's stage, 128 B of every row at a time, so
+            // that the stores are whole lines
+            const int64_t my_off = final ? ((int64_t)(t0 + tok) * p.r.o_tok +
+                                            (int64_t)head * p.r.o_head) * 2
+                                         : part_at * (PR_HD * 4);
+            uint8_t* dst = final ? reinterpret_cast<uint8_t*>(p.r.out)
+                                 : reinterpret_cast<uint8_t*>(p.parts_out);
+            const bool any = __any_sync(0xffffffffu, l > 0.f);
+            uint8_t* stage = sm.stage[warp];
+            const int live = min(n_rows - (by_rows ? i * TA_TILE : 0) - q4 * 32, 32);
+            int64_t off[8];
 #pragma unroll
-                    for (int e = 0; e < 32; e += 4) {
-                        float f[4];
+            for (int k = 0; k < 8; ++k)
+                off[k] = __shfl_sync(0xffffffffu, my_off, 4 * k + (lane >> 3)) + 16 * (lane & 7);
+            auto send = [&](int byte) {             // bytes [byte, byte + 128) of the rows
+                __syncwarp();
+                uint4 x[8];
 #pragma unroll
-                        for (int x = 0; x < 4; ++x) {
-                            f[x] = l > 0.f && w0 > 0.f ? w0 * __uint_as_float(o[e + x]) : 0.f;
-                            if (second)
-                                f[x] += w1 * xo[(32 * c + e + x) * TA_TILE + q4 * 32 + lane];
-                        }
-                        if (local < n_rows)
-                            *reinterpret_cast<float4*>(out + 32 * c + e) =
-                                make_float4(f[0], f[1], f[2], f[3]);
+                for (int k = 0; k < 8; ++k)
+                    x[k] = *reinterpret_cast<const uint4*>(
+                        stage + tc_swz(4 * k + (lane >> 3), 16 * (lane & 7)));
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    if (4 * k + (lane >> 3) < live)
+                        *reinterpret_cast<uint4*>(dst + off[k] + byte) = x[k];
+                __syncwarp();
+            };
+            if (final || any) {
+                for (int c = chunk0; c < chunk0 + chunks; ++c) {
+                    uint32_t o[32];
+                    float f[32];
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) f[e] = 0.f;
+                    tc_ld32(lane_base + TM_O + i * PR_HD + 32 * c, o);
+                    tc_wait_ld();
+                    tc_tie32(o);
+                    // (without a product there is no O)
+                    if (w_mine > 0.f)
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) f[e] = w_mine * __uint_as_float(o[e]);
+                    if (!by_rows) {
+                        tc_ld32(lane_base + TM_O + (1 - i) * PR_HD + 32 * c, o);
+                        tc_wait_ld();
+                        tc_tie32(o);
+                        if (w_other > 0.f)
+#pragma unroll
+                            for (int e = 0; e < 32; ++e)
+                                f[e] = fmaf(w_other, __uint_as_float(o[e]), f[e]);
+                    }
+                    if (final) {
+#pragma unroll
+                        for (int e = 0; e < 32; e += 8)
+                            *reinterpret_cast<uint4*>(
+                                stage + tc_swz(lane, (c & 1) * 64 + 2 * e)) =
+                                make_uint4(pack_bf16x2(f[e], f[e + 1]), pack_bf16x2(f[e + 2], f[e + 3]),
+                                           pack_bf16x2(f[e + 4], f[e + 5]), pack_bf16x2(f[e + 6], f[e + 7]));
+                        if (c & 1) send((c >> 1) * 128);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 32; e += 4)
+                            *reinterpret_cast<float4*>(stage + tc_swz(lane, 4 * e)) =
+                                make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
+                        send(c * 128);
                     }
                 }
             }
-            if (local < n_rows)
-                *reinterpret_cast<float2*>(p.parts_ml + 2 * at) =
-                    make_float2(l > 0.f ? m * sl2 : -INFINITY, l);
+            if (local < n_rows && (by_rows || i == 0)) {
+                if (!final)         // O is relative to m; (m in log2 units, l)
+                    *reinterpret_cast<float2*>(p.parts_ml + 2 * part_at) =
+                        make_float2(l > 0.f ? m * sl2 : -INFINITY, l);
+                else if (p.r.lse)
+                    p.r.lse[(int64_t)(t0 + tok) * p.r.lse_tok + head] =
+                        l > 0.f ? (m * sl2 + log2f(l)) * PR_LN2 : -INFINITY;
+            }
+            tc_before_sync();
+            // (the other stream has read this one's O and sums before they change)
+            if (!by_rows) asm volatile("bar.sync 1, 256;" ::: "memory");
         }
-        tc_before_sync();
     }
     __syncwarp();
     __syncthreads();
@@ -648,6 +794,7 @@ __global__ void __launch_bounds__(32 * TJ_WARPS) join_parts_kernel(const TileAtt
 
 int launch_tile_attn(const char* who, TileAttnParams p, int max_tiles, cudaStream_t s) {
     p.head_chunks = p.r.n_kv > 1 ? (int)(p.r.sh / 64) : 0;
+    p.max_tiles = max_tiles;
     CUtensorMap mk, mv;
     CUresult cr = encode_plane(&mk, p.r.k, p.r.n_kv, p.r.num_blocks, 64 * p.head_chunks, p.r.st, p.r.sb);
     if (cr == CUDA_SUCCESS)
@@ -664,7 +811,10 @@ int launch_tile_attn(const char* who, TileAttnParams p, int max_tiles, cudaStrea
                              smem);
         attr_done[dev] = true;
     }
-    tile_attn_kernel<<<dim3(max_tiles, p.r.n_kv, p.parts), TA_THREADS, smem, s>>>(mk, mv, p);
+    const int64_t items = (int64_t)max_tiles * p.r.n_kv * p.parts;
+    LOCKS_REQUIRE(items < (1 << 30), LOCKS_ERR_SIZE, "%s: too many query rows in one call", who);
+    tile_attn_kernel<<<(int)(items < sm_count() ? items : sm_count()), TA_THREADS, smem, s>>>(
+        mk, mv, p);
     return check_launch(who);
 }
 
