@@ -52,9 +52,11 @@ constexpr int TA_BYTES = 2 * TA_HALF;
 constexpr int TA_BOX = PR_PAGE * 256;              // bytes of a page of one plane and head
 constexpr int TM_S = 0, TM_O = 256, TM_COLS = 512;
 constexpr float TA_RAISE = 8.f;
+// one pair of exponentials in TA_POLY leaves the special-function unit alone
+constexpr int TA_POLY = 4;
 // P is handed over in two steps, so that the product of the first is under way while
 // the exponentials of the second are taken
-constexpr int TA_EARLY = 6;                        // pages (k-steps) of the first step
+constexpr int TA_EARLY = 4;                        // pages (k-steps) of the first step
 
 struct Item {
     int valid, seg, kh, part, t0, row0, n_rows, j0, n_tiles, key_end, written, base_pos;
@@ -96,6 +98,27 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
         : "=l"(reinterpret_cast<uint64_t&>(d))
         : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
     return d;
+}
+
+// 2^x of a pair on the multiply-add pipe, x <= 127: 2^n 2^f with n the nearest whole
+// number (read off the low bits of x + 1.5 2^23) and 1 + f q(f), |f| <= 1/2, q of degree
+// 3 (own minimax fit, relative error 2.8e-6: P is rounded to 8 bits anyway, and the
+// sum's error stays below that).  Below -127, where a hidden key's -inf lands, it is
+// exactly 0, because the polynomial is exactly 1 at f = 0.
+__device__ __forceinline__ float2 exp2_poly(float2 x) {
+    x.x = fmaxf(x.x, -127.f);
+    x.y = fmaxf(x.y, -127.f);
+    const float2 t = add2(x, make_float2(12582912.f, 12582912.f));
+    const float2 n = add2(t, make_float2(-12582912.f, -12582912.f));
+    const float2 f = fma2(n, make_float2(-1.f, -1.f), x);
+    float2 r = make_float2(0x1.3a02ccp-7f, 0x1.3a02ccp-7f);
+    r = fma2(r, f, make_float2(0x1.c9fc46p-5f, 0x1.c9fc46p-5f));
+    r = fma2(r, f, make_float2(0x1.ec0378p-3f, 0x1.ec0378p-3f));
+    r = fma2(r, f, make_float2(0x1.62e12cp-1f, 0x1.62e12cp-1f));
+    r = fma2(r, f, make_float2(1.f, 1.f));
+    r.x = __int_as_float(__float_as_int(r.x) + (__float_as_int(t.x) << 23));
+    r.y = __int_as_float(__float_as_int(r.y) + (__float_as_int(t.y) << 23));
+    return r;
 }
 
 // a wait that gives up once any wait of the CTA has
@@ -617,8 +640,12 @@ tile_attn_kernel(const __grid_constant__ CUtensorMap map_k,
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
                         float2 x = fma2(make_float2(s[32 * c + 2 * e], s[32 * c + 2 * e + 1]), k2, b2);
-                        x.x = pr_exp2(x.x);
-                        x.y = pr_exp2(x.y);
+                        if (e % TA_POLY == TA_POLY - 1) {
+                            x = exp2_poly(x);
+                        } else {
+                            x.x = pr_exp2(x.x);
+                            x.y = pr_exp2(x.y);
+                        }
                         sum[e & 1] = add2(sum[e & 1], x);
                         pk[e] = pack_bf16x2(x.x, x.y);
                     }
