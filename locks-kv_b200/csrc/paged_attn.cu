@@ -88,7 +88,7 @@ extern "C" int locks_window_attention(
         // bound of the tiles, CTAs without one return at once)
         const int64_t rows = (int64_t)n_tok * G;
         const int64_t many = rows / (FEW_ROWS + 1) < n_req ? rows / (FEW_ROWS + 1) : n_req;
-        int64_t tiles = rows / TILE_ROWS + many;
+        int64_t tiles = (rows + (TILE_ROWS - 1) * many) / TILE_ROWS;
         const int64_t most = many * (((int64_t)max_q * G + TILE_ROWS - 1) / TILE_ROWS);
         tiles = tiles < most ? tiles : most;
         if (tiles > 0) {
@@ -105,12 +105,15 @@ extern "C" int locks_window_attention(
                 tp.parts_out = scratch;
                 tp.parts_ml = scratch + tp.parts * tp.part_rows * PR_HD;
             }
+            p.beside = 1;
             int rc2 = launch_tile_attn(who, tp, (int)tiles, s);
+            if (rc2 == LOCKS_OK)
+                rc2 = launch_row_attn(who, p, n_req, max_q < FEW_ROWS ? max_q * G : FEW_ROWS, s);
             if (rc2 == LOCKS_OK && tp.parts > 1) rc2 = launch_join_parts(who, tp, n_tok, s);
-            if (rc2 != LOCKS_OK) return rc2;
+            return rc2;
         }
     }
-    return launch_row_attn(who, p, n_req, s);
+    return launch_row_attn(who, p, n_req, max_q < FEW_ROWS ? max_q * G : FEW_ROWS, s);
 }
 
 extern "C" int locks_shared_prefix_decode(
@@ -150,7 +153,10 @@ extern "C" int locks_shared_prefix_decode(
     tp.r = p;
     tp.bounds = cu_groups; tp.prefix_lens = prefix_lens; tp.n_seg = n_groups;
     tp.status = status;
-    const int64_t tiles = (int64_t)n_req * G / TILE_ROWS + (n_groups < n_req ? n_groups : n_req);
+    // upper bound of the groups' row tiles (each group rounds up once)
+    const int64_t tiles = ((int64_t)n_req * G +
+                           (int64_t)(TILE_ROWS - 1) * (n_groups < n_req ? n_groups : n_req)) /
+                          TILE_ROWS;
     tp.part_rows = (int64_t)n_req * n_kv * G;
     tp.parts = parts_for(tiles * n_kv, bt_width, tp.part_rows * (PR_HD + 2), scratch_floats);
     tp.parts_out = scratch;
@@ -158,7 +164,8 @@ extern "C" int locks_shared_prefix_decode(
     const int rc2 = launch_tile_attn(who, tp, (int)tiles, s);
     if (rc2 != LOCKS_OK) return rc2;
     p.max_rows = FEW_ROWS;
+    p.beside = 1;
     p.parts = tp.parts; p.part_rows = tp.part_rows;
     p.parts_o = tp.parts_out; p.parts_ml = tp.parts_ml;
-    return launch_row_attn(who, p, n_req, s);
+    return launch_row_attn(who, p, n_req, G, s);
 }

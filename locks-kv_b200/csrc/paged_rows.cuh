@@ -31,6 +31,11 @@ struct PageList {
         // (pos - key < window: no overflow for key >= 0, pos < 2^31)
         return key <= pos && key < key_end && (pos - key < window || key < sinks);
     }
+    // whether all of the queries see the whole page
+    __device__ __forceinline__ bool all_see(int pg) const {
+        const int first = pg * PR_PAGE, last = first + PR_PAGE - 1;
+        return last <= pos_lo && last < key_end && (pos_hi - first < window || last < sinks);
+    }
     // whether any of the queries sees the key: the last one sees the newest keys,
     // the first one's window reaches back furthest
     __device__ __forceinline__ bool any_sees(int key) const {
@@ -67,18 +72,17 @@ __device__ __forceinline__ PartSum join_parts(const float* o, const float* ml, i
                                               int parts, int64_t at, int d) {
     PartSum r = {-INFINITY, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
 #pragma unroll 4
+    for (int s = 0; s < parts; ++s) r.m = fmaxf(r.m, ml[2 * (s * rows + at)]);
+    // (loads that do not depend on one another; a part without keys has -inf and no O)
+#pragma unroll 4
     for (int s = 0; s < parts; ++s) {
         const int64_t i = s * rows + at;
         const float2 x = *reinterpret_cast<const float2*>(ml + 2 * i);
-        if (x.y > 0.f) {
-            const float4 v = *reinterpret_cast<const float4*>(o + i * PR_HD + d);
-            const float up = fmaxf(r.m, x.x);
-            const float a = pr_exp2(r.m - up), b = pr_exp2(x.x - up);
-            r.l = a * r.l + b * x.y;
-            r.o.x = a * r.o.x + b * v.x; r.o.y = a * r.o.y + b * v.y;
-            r.o.z = a * r.o.z + b * v.z; r.o.w = a * r.o.w + b * v.w;
-            r.m = up;
-        }
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (x.y > 0.f) v = *reinterpret_cast<const float4*>(o + i * PR_HD + d);
+        const float w = x.y > 0.f ? pr_exp2(x.x - r.m) : 0.f;
+        r.l += w * x.y;
+        r.o.x += w * v.x; r.o.y += w * v.y; r.o.z += w * v.z; r.o.w += w * v.w;
     }
     return r;
 }
@@ -101,6 +105,7 @@ struct RowAttnParams {
     int n_kv, G, window, sinks;
     float scale_log2;                 // softmax scale * log2(e)
     int max_rows;                     // requests with more rows (tokens x G) are left out
+    int beside;                       // the launch before this one is the call's tiled kernel
     // shared prefix: (n_groups + 1) row bounds, or null; the whole pages of the prefix
     // are in `parts` partial results already (layout: TileAttnParams)
     const int32_t* cu_groups;
@@ -126,8 +131,10 @@ struct TileAttnParams {
     int max_tiles;                    // upper bound of the row tiles of all segments
 };
 
-// csrc/row_attn.cu; `who` names the entry point in error messages
-int launch_row_attn(const char* who, const RowAttnParams& p, int n_req, cudaStream_t s);
+// csrc/row_attn.cu; `who` names the entry point in error messages, no request has more
+// than most_rows rows that the launch has to serve
+int launch_row_attn(const char* who, const RowAttnParams& p, int n_req, int most_rows,
+                    cudaStream_t s);
 // csrc/tile_attn.cu
 int launch_tile_attn(const char* who, TileAttnParams p, int max_tiles, cudaStream_t s);
 int launch_join_parts(const char* who, const TileAttnParams& p, int n_tok, cudaStream_t s);

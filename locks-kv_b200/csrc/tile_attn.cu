@@ -259,6 +259,7 @@ tile_attn_kernel(const __grid_constant__ CUtensorMap map_k,
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
         tc_before_sync();
     }
+    pdl_trigger();                      // the call's next launch may take SMs as they free up
     __syncthreads();
     tc_after_sync();
     const uint32_t tmem = sm.tmem_base;
@@ -800,6 +801,7 @@ __global__ void __launch_bounds__(32 * TJ_WARPS) join_parts_kernel(const TileAtt
     const int lane = threadIdx.x & 31, H = p.r.n_kv * p.r.G;
     const int64_t at = (int64_t)blockIdx.x * TJ_WARPS + (threadIdx.x >> 5);
     const int tok = (int)(at / H), h = (int)(at - (int64_t)tok * H);
+    pdl_wait();
     if (tok >= n_tok || tok < p.bounds[0] || tok >= p.bounds[p.n_seg]) return;
     int lo = 0, hi = p.n_seg - 1;                   // the token's request
     while (lo < hi) {
@@ -847,8 +849,18 @@ int launch_tile_attn(const char* who, TileAttnParams p, int max_tiles, cudaStrea
 
 int launch_join_parts(const char* who, const TileAttnParams& p, int n_tok, cudaStream_t s) {
     const int64_t rows = (int64_t)n_tok * p.r.n_kv * p.r.G;
-    join_parts_kernel<<<(unsigned)((rows + TJ_WARPS - 1) / TJ_WARPS), 32 * TJ_WARPS, 0, s>>>(
-        p, n_tok);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)((rows + TJ_WARPS - 1) / TJ_WARPS), 1, 1);
+    cfg.blockDim = dim3(32 * TJ_WARPS, 1, 1);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl_enabled() ? 1 : 0;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, join_parts_kernel, p, n_tok);
+    if (e != cudaSuccess)
+        return fail(LOCKS_ERR_LAUNCH, "%s: %s", who, cudaGetErrorString(e));
     return check_launch(who);
 }
 
