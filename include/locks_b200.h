@@ -636,8 +636,8 @@ int locks_dense_decode(const void* q, int64_t q_stride_req, const void* k_cache,
  * read by each request itself).  Results equal attention of every request over
  * its own table.  Rows outside the groups are left as they were; a request with
  * seq_lens[r] <= 0 gets 0.  scratch (fp32, scratch_floats of them): at least
- * n_req * n_kv * G * (head_dim + 2); more lets a long prefix be cut into more
- * parts. */
+ * 2 * n_req * n_kv * G * (head_dim + 2); more lets a long prefix be cut into more
+ * parts (as many as the device has room for, one such half each). */
 int locks_append_plan(const int32_t* seq_lens, const int32_t* n_new,
                       int32_t* block_table, int64_t bt_stride, int bt_width,
                       const int32_t* free_blocks, int n_free, const int32_t* taken,

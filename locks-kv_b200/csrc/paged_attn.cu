@@ -106,10 +106,10 @@ extern "C" int locks_window_attention(
                 tp.parts_ml = scratch + tp.parts * tp.part_rows * PR_HD;
             }
             p.beside = 1;
-            int rc2 = launch_tile_attn(who, tp, (int)tiles, s);
+            int rc2 = launch_tile_attn(who, tp, (int)tiles, n_tok, s);
             if (rc2 == LOCKS_OK)
                 rc2 = launch_row_attn(who, p, n_req, max_q < FEW_ROWS ? max_q * G : FEW_ROWS, s);
-            if (rc2 == LOCKS_OK && tp.parts > 1) rc2 = launch_join_parts(who, tp, n_tok, s);
+            if (rc2 == LOCKS_OK && tp.parts > 1) rc2 = launch_join_parts(who, tp, tp.parts, n_tok, s);
             return rc2;
         }
     }
@@ -143,9 +143,9 @@ extern "C" int locks_shared_prefix_decode(
     LOCKS_REQUIRE(cu_groups && prefix_lens && scratch, LOCKS_ERR_ARG,
                   "%s: null pointer argument", who);
     LOCKS_REQUIRE(n_groups >= 0, LOCKS_ERR_ARG, "%s: bad size argument", who);
-    LOCKS_REQUIRE(scratch_floats >= (int64_t)n_req * n_kv * G * (PR_HD + 2), LOCKS_ERR_SIZE,
+    LOCKS_REQUIRE(scratch_floats >= (int64_t)n_req * n_kv * G * (PR_HD + 2) * 2, LOCKS_ERR_SIZE,
                   "%s: scratch holds %lld floats, at least %lld are needed", who,
-                  (long long)scratch_floats, (long long)n_req * n_kv * G * (PR_HD + 2));
+                  (long long)scratch_floats, (long long)n_req * n_kv * G * (PR_HD + 2) * 2);
     LOCKS_REQUIRE(scale > 0.f, LOCKS_ERR_ARG, "%s: scale must be positive", who);
     if (n_req == 0 || n_groups == 0) return LOCKS_OK;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -158,14 +158,17 @@ extern "C" int locks_shared_prefix_decode(
                            (int64_t)(TILE_ROWS - 1) * (n_groups < n_req ? n_groups : n_req)) /
                           TILE_ROWS;
     tp.part_rows = (int64_t)n_req * n_kv * G;
-    tp.parts = parts_for(tiles * n_kv, bt_width, tp.part_rows * (PR_HD + 2), scratch_floats);
+    // (one part more for the requests' own keys)
+    const int64_t part_floats = tp.part_rows * (PR_HD + 2);
+    tp.parts = parts_for(tiles * n_kv, bt_width, part_floats, scratch_floats - part_floats);
     tp.parts_out = scratch;
-    tp.parts_ml = scratch + tp.parts * tp.part_rows * PR_HD;
-    const int rc2 = launch_tile_attn(who, tp, (int)tiles, s);
-    if (rc2 != LOCKS_OK) return rc2;
+    tp.parts_ml = scratch + (tp.parts + 1) * tp.part_rows * PR_HD;
     p.max_rows = FEW_ROWS;
     p.beside = 1;
-    p.parts = tp.parts; p.part_rows = tp.part_rows;
+    p.part = tp.parts; p.part_rows = tp.part_rows;
     p.parts_o = tp.parts_out; p.parts_ml = tp.parts_ml;
-    return launch_row_attn(who, p, n_req, G, s);
+    int rc2 = launch_tile_attn(who, tp, (int)tiles, n_req, s);
+    if (rc2 == LOCKS_OK) rc2 = launch_row_attn(who, p, n_req, G, s);
+    if (rc2 == LOCKS_OK) rc2 = launch_join_parts(who, tp, tp.parts + 1, n_req, s);
+    return rc2;
 }

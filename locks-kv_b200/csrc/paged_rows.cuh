@@ -71,18 +71,35 @@ struct PartSum {
 __device__ __forceinline__ PartSum join_parts(const float* o, const float* ml, int64_t rows,
                                               int parts, int64_t at, int d) {
     PartSum r = {-INFINITY, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
-#pragma unroll 4
-    for (int s = 0; s < parts; ++s) r.m = fmaxf(r.m, ml[2 * (s * rows + at)]);
-    // (loads that do not depend on one another; a part without keys has -inf and no O)
-#pragma unroll 4
-    for (int s = 0; s < parts; ++s) {
-        const int64_t i = s * rows + at;
-        const float2 x = *reinterpret_cast<const float2*>(ml + 2 * i);
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (x.y > 0.f) v = *reinterpret_cast<const float4*>(o + i * PR_HD + d);
-        const float w = x.y > 0.f ? pr_exp2(x.x - r.m) : 0.f;
-        r.l += w * x.y;
-        r.o.x += w * v.x; r.o.y += w * v.y; r.o.z += w * v.z; r.o.w += w * v.w;
+    // eight parts' loads in flight at a time, none waiting for another
+    for (int s0 = 0; s0 < parts; s0 += 8) {
+        float2 x[8];
+        float4 v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const int64_t i = (int64_t)min(s0 + k, parts - 1) * rows + at;
+            x[k] = *reinterpret_cast<const float2*>(ml + 2 * i);
+            v[k] = *reinterpret_cast<const float4*>(o + i * PR_HD + d);
+        }
+        float up = r.m;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            if (s0 + k >= parts) x[k].y = 0.f;
+            if (x[k].y > 0.f) up = fmaxf(up, x[k].x);
+        }
+        const float a = r.l > 0.f ? pr_exp2(r.m - up) : 0.f;
+        r.l *= a;
+        r.o.x *= a; r.o.y *= a; r.o.z *= a; r.o.w *= a;
+        r.m = up;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            if (x[k].y > 0.f) {                 // (a part without keys wrote no O)
+                const float w = pr_exp2(x[k].x - up);
+                r.l += w * x[k].y;
+                r.o.x += w * v[k].x; r.o.y += w * v[k].y;
+                r.o.z += w * v[k].z; r.o.w += w * v[k].w;
+            }
+        }
     }
     return r;
 }
@@ -106,13 +123,13 @@ struct RowAttnParams {
     float scale_log2;                 // softmax scale * log2(e)
     int max_rows;                     // requests with more rows (tokens x G) are left out
     int beside;                       // the launch before this one is the call's tiled kernel
-    // shared prefix: (n_groups + 1) row bounds, or null; the whole pages of the prefix
-    // are in `parts` partial results already (layout: TileAttnParams)
+    // shared prefix: (n_groups + 1) row bounds, or null; the whole pages of the prefix are
+    // left out, and the result becomes part number `part` (layout: TileAttnParams)
     const int32_t* cu_groups;
     const int32_t* prefix_lens;
-    int n_groups, parts;
+    int n_groups, part;
     int64_t part_rows;
-    const float *parts_o, *parts_ml;
+    float *parts_o, *parts_ml;
 };
 
 // the tiled kernel: segments bounds[s] .. bounds[s + 1] of query tokens
@@ -136,7 +153,9 @@ struct TileAttnParams {
 int launch_row_attn(const char* who, const RowAttnParams& p, int n_req, int most_rows,
                     cudaStream_t s);
 // csrc/tile_attn.cu
-int launch_tile_attn(const char* who, TileAttnParams p, int max_tiles, cudaStream_t s);
-int launch_join_parts(const char* who, const TileAttnParams& p, int n_tok, cudaStream_t s);
+int launch_tile_attn(const char* who, TileAttnParams p, int max_tiles, int n_tok,
+                     cudaStream_t s);
+int launch_join_parts(const char* who, const TileAttnParams& p, int parts, int n_tok,
+                      cudaStream_t s);
 
 }  // namespace locks

@@ -30,8 +30,7 @@
 //
 // Behind the tiled kernel of the same call it is launched programmatically: it starts on
 // SMs that have run out of tiles (the tiled kernel lets it once all of its CTAs run, when
-// everything earlier on the stream is done) and waits for that kernel only before it reads
-// partial results, or before it ends.
+// everything earlier on the stream is done) and waits for that kernel only before it ends.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -322,18 +321,13 @@ __global__ void __launch_bounds__(WARPS * 32) row_attn_kernel(const RowAttnParam
         };
         auto finish = [&](int row, int d, float M, float L, float4 o) {
             const int at = rb * 16 + row, i = at / G, h = kh * G + at - i * G;
-            if (p.parts) {
-                // (one query token per request: i == 0, tok0 == r)
-                const int64_t pr = (int64_t)tok0 * p.n_kv * G + h;
-                const PartSum s = join_parts(p.parts_o, p.parts_ml, p.part_rows, p.parts, pr, d);
-                if (s.l > 0.f) {
-                    const float up = fmaxf(M, s.m);
-                    const float a = L > 0.f ? pr_exp2(M - up) : 0.f, b = pr_exp2(s.m - up);
-                    L = a * L + b * s.l;
-                    o = make_float4(a * o.x, a * o.y, a * o.z, a * o.w);
-                    axpy4(o, b, s.o);
-                    M = up;
-                }
+            if (p.parts_o) {
+                // one of several parts (one query token per request: i == 0, tok0 == r)
+                const int64_t x = p.part * p.part_rows + (int64_t)tok0 * p.n_kv * G + h;
+                *reinterpret_cast<float4*>(p.parts_o + x * PR_HD + d) = o;
+                if (d == 0)
+                    *reinterpret_cast<float2*>(p.parts_ml + 2 * x) = make_float2(M, L);
+                return;
             }
             const float inv = L > 0.f ? 1.f / L : 0.f;
             *reinterpret_cast<uint2*>(p.out + (int64_t)(tok0 + i) * p.o_tok +
@@ -343,7 +337,6 @@ __global__ void __launch_bounds__(WARPS * 32) row_attn_kernel(const RowAttnParam
                 p.lse[(int64_t)(tok0 + i) * p.lse_tok + h] =
                     L > 0.f ? (M + log2f(L)) * PR_LN2 : -INFINITY;
         };
-        if (p.parts) pdl_wait();                // the partial results are the tiled kernel's
         if (!CLUSTER) {
             for (int e = tid; e < n_el; e += THREADS) {
                 float M, L;

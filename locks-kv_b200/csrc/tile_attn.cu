@@ -162,6 +162,15 @@ __device__ __forceinline__ void tma_load_page(void* dst, const CUtensorMap* map,
         : "memory");
 }
 
+__device__ __forceinline__ void tma_load_rows(void* dst, const CUtensorMap* map, int channel,
+                                              int head, int token, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes "
+        "[%0], [%1, {%2, %3, %4}], [%5];"
+        ::"r"(smem_u32(dst)), "l"(map), "r"(channel), "r"(head), "r"(token), "r"(smem_u32(bar))
+        : "memory");
+}
+
 // segment s: first token and token count (0 where the few-row kernel serves it)
 __device__ __forceinline__ void segment(const TileAttnParams& p, int s, int& t0, int& n) {
     t0 = p.bounds[s];
@@ -176,8 +185,11 @@ __device__ __forceinline__ bool find_item(const TileAttnParams& p, int w, int la
     const int target = w % p.max_tiles, rest = w / p.max_tiles;
     int before = 0;
     for (int s0 = 0; s0 < p.n_seg; s0 += 32) {
-        int t0 = 0, n = 0;
-        if (s0 + lane < p.n_seg) segment(p, s0 + lane, t0, n);
+        int t0 = 0, n = 0, extent = 0;
+        if (s0 + lane < p.n_seg) {
+            extent = p.prefix_lens ? p.prefix_lens[s0 + lane] : p.r.seq_lens[s0 + lane];
+            segment(p, s0 + lane, t0, n);
+        }
         const int mine = (n * p.r.G + 2 * TA_TILE - 1) / (2 * TA_TILE);
         int x = mine;
 #pragma unroll
@@ -192,6 +204,7 @@ __device__ __forceinline__ bool find_item(const TileAttnParams& p, int w, int la
             it.seg = s0 + src;
             it.t0 = __shfl_sync(0xffffffffu, t0, src);
             n = __shfl_sync(0xffffffffu, n, src);
+            extent = __shfl_sync(0xffffffffu, extent, src);
             // longest rows first
             const int tile = __shfl_sync(0xffffffffu, mine - 1 - (target - from), src);
             const int G = p.r.G;
@@ -201,12 +214,12 @@ __device__ __forceinline__ bool find_item(const TileAttnParams& p, int w, int la
             it.n_rows = min(n * G - it.row0, 2 * TA_TILE);
             it.base_pos = 0;
             if (p.prefix_lens) {
-                const int whole = min(max(p.prefix_lens[it.seg], 0) / PR_PAGE, p.r.bt_width);
+                const int whole = min(max(extent, 0) / PR_PAGE, p.r.bt_width);
                 it.written = it.key_end = whole * PR_PAGE;
                 it.table_row = it.t0;
                 it.list = page_list(0, it.key_end - 1, INT32_MAX, 0, p.r.bt_width);
             } else {
-                it.written = p.r.seq_lens[it.seg];
+                it.written = extent;
                 it.base_pos = it.written - n;
                 it.table_row = it.seg;
                 it.list = page_list(it.base_pos + it.row0 / G,
@@ -227,7 +240,8 @@ __device__ __forceinline__ bool find_item(const TileAttnParams& p, int w, int la
 }
 
 __global__ void __launch_bounds__(TA_THREADS, 1)
-tile_attn_kernel(const __grid_constant__ CUtensorMap map_k,
+tile_attn_kernel(const __grid_constant__ CUtensorMap map_q,
+                 const __grid_constant__ CUtensorMap map_k,
                  const __grid_constant__ CUtensorMap map_v, const TileAttnParams p) {
     extern __shared__ uint8_t ta_raw[];
     TileSmem& sm = *reinterpret_cast<TileSmem*>(
@@ -298,7 +312,7 @@ tile_attn_kernel(const __grid_constant__ CUtensorMap map_k,
             }
         } else if (warp == 11) {
             // ---- Q into the swizzled K-major layout, 16 lanes to a row -------------------
-            int loads = 0;
+            int loads = 0, both = 0;
             for (int n = 0;; ++n) {
                 const Item* item = next_item(n);
                 if (!item) break;
@@ -309,17 +323,32 @@ tile_attn_kernel(const __grid_constant__ CUtensorMap map_k,
                 if (loads > 0)
                     ta_wait(sm, &sm.q_empty, (uint32_t)(loads - 1) & 1u, p.status);
                 ++loads;
+                const int subs = n_rows > TA_TILE ? 2 : 1;
+                both += subs - 1;
+                if (TA_TILE % G == 0) {
+                    // a stream's rows are whole tokens: one box for each half of the
+                    // channels (rows behind the last one are somebody else's or zeros:
+                    // a row only reaches its own output, which is not stored)
+                    if (lane == 0)
+                        for (int sub = 0; sub < subs; ++sub) {
+                            mbar_expect_tx(&sm.q_full[sub], TA_BYTES);
+                            for (int half = 0; half < 2; ++half)
+                                tma_load_rows(&sm.q[sub][half * TA_HALF], &map_q, 64 * half, kh * G,
+                                              t0 + (row0 + sub * TA_TILE) / G, &sm.q_full[sub]);
+                        }
+                    __syncwarp();
+                    continue;
+                }
                 // (rows behind the last one are zeros; every copy is on its way before
                 // the first is waited for)
                 const int piece = lane & 15;
                 int row = lane >> 4, tok = (row0 + row) / G, g = row0 + row - tok * G;
                 const __nv_bfloat16* src = p.r.q + (int64_t)(t0 + tok) * p.r.q_tok +
                                            (int64_t)(kh * G + g) * p.r.q_head + 8 * piece;
-                // two rows on: in the same token, or in the next one (G = 1: the one after)
-                const int64_t stay = 2 * p.r.q_head,
-                              wrap = G == 1 ? 2 * p.r.q_tok : p.r.q_tok + (2 - G) * p.r.q_head;
+                // two rows on: in the same token, or in the next one
+                const int64_t stay = 2 * p.r.q_head, wrap = p.r.q_tok + (2 - G) * p.r.q_head;
                 const uint32_t d0 = smem_u32(sm.q) + (piece >> 3) * TA_HALF;
-                for (int sub = 0; sub < (n_rows > TA_TILE ? 2 : 1); ++sub) {
+                for (int sub = 0; sub < subs; ++sub) {
 #pragma unroll 8
                     for (int k = 0; k < TA_TILE / 2; ++k) {
                         const bool live = row < n_rows;
@@ -328,7 +357,7 @@ tile_attn_kernel(const __grid_constant__ CUtensorMap map_k,
                                    live ? src : p.r.q, live ? 16 : 0);
                         const bool over = g + 2 >= G;
                         src += over ? wrap : stay;
-                        g = G == 1 ? 0 : g + 2 - (over ? G : 0);
+                        g += 2 - (over ? G : 0);
                         row += 2;
                     }
                     asm volatile("cp.async.wait_all;" ::: "memory");
@@ -336,6 +365,10 @@ tile_attn_kernel(const __grid_constant__ CUtensorMap map_k,
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&sm.q_full[sub]);
                 }
+            }
+            if (__any_sync(0xffffffffu, is_dead(sm))) {     // copies in flight land first
+                if (loads > 0) mbar_wait(&sm.q_full[0], (uint32_t)(loads - 1) & 1u, p.status);
+                if (both > 0) mbar_wait(&sm.q_full[1], (uint32_t)(both - 1) & 1u, p.status);
             }
         } else if (warp == 9) {
             // ---- pages: K and V tiles in the order the products take them ---------------
@@ -716,42 +749,51 @@ tile_attn_kernel(const __grid_constant__ CUtensorMap map_k,
                         *reinterpret_cast<uint4*>(dst + off[k] + byte) = x[k];
                 __syncwarp();
             };
+            // 128 columns of tensor memory: all of this stream's O, or the same 64 of both
+            uint32_t o[TA_TILE];
+            float* f = reinterpret_cast<float*>(o);
             if (final || any) {
-                for (int c = chunk0; c < chunk0 + chunks; ++c) {
-                    uint32_t o[32];
-                    float f[32];
+                const uint32_t here = lane_base + TM_O + i * PR_HD + 32 * chunk0;
+                const uint32_t there =
+                    by_rows ? here + 64 : lane_base + TM_O + (1 - i) * PR_HD + 32 * chunk0;
+                tc_ld32(here, o);
+                tc_ld32(here + 32, o + 32);
+                tc_ld32(there, o + 64);
+                tc_ld32(there + 32, o + 96);
+                tc_wait_ld();
+                tc_tie32(o);
+                tc_tie32(o + 32);
+                tc_tie32(o + 64);
+                tc_tie32(o + 96);
+                // (without a product there is no O)
+                const float w2 = by_rows ? w_mine : w_other;
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) f[e] = 0.f;
-                    tc_ld32(lane_base + TM_O + i * PR_HD + 32 * c, o);
-                    tc_wait_ld();
-                    tc_tie32(o);
-                    // (without a product there is no O)
-                    if (w_mine > 0.f)
+                for (int e = 0; e < 64; ++e) {
+                    f[e] = w_mine > 0.f ? w_mine * f[e] : 0.f;
+                    f[64 + e] = w2 > 0.f ? w2 * f[64 + e] : 0.f;
+                }
+                if (!by_rows)
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) f[e] = w_mine * __uint_as_float(o[e]);
-                    if (!by_rows) {
-                        tc_ld32(lane_base + TM_O + (1 - i) * PR_HD + 32 * c, o);
-                        tc_wait_ld();
-                        tc_tie32(o);
-                        if (w_other > 0.f)
+                    for (int e = 0; e < 64; ++e) f[e] += f[64 + e];
 #pragma unroll
-                            for (int e = 0; e < 32; ++e)
-                                f[e] = fmaf(w_other, __uint_as_float(o[e]), f[e]);
-                    }
+                for (int c = 0; c < 4; ++c) {
+                    if (c >= chunks) break;
                     if (final) {
 #pragma unroll
                         for (int e = 0; e < 32; e += 8)
-                            *reinterpret_cast<uint4*>(
-                                stage + tc_swz(lane, (c & 1) * 64 + 2 * e)) =
-                                make_uint4(pack_bf16x2(f[e], f[e + 1]), pack_bf16x2(f[e + 2], f[e + 3]),
-                                           pack_bf16x2(f[e + 4], f[e + 5]), pack_bf16x2(f[e + 6], f[e + 7]));
-                        if (c & 1) send((c >> 1) * 128);
+                            *reinterpret_cast<uint4*>(stage + tc_swz(lane, (c & 1) * 64 + 2 * e)) =
+                                make_uint4(pack_bf16x2(f[32 * c + e], f[32 * c + e + 1]),
+                                           pack_bf16x2(f[32 * c + e + 2], f[32 * c + e + 3]),
+                                           pack_bf16x2(f[32 * c + e + 4], f[32 * c + e + 5]),
+                                           pack_bf16x2(f[32 * c + e + 6], f[32 * c + e + 7]));
+                        if (c & 1) send(((chunk0 + c) >> 1) * 128);
                     } else {
 #pragma unroll
                         for (int e = 0; e < 32; e += 4)
                             *reinterpret_cast<float4*>(stage + tc_swz(lane, 4 * e)) =
-                                make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
-                        send(c * 128);
+                                make_float4(f[32 * c + e], f[32 * c + e + 1], f[32 * c + e + 2],
+                                            f[32 * c + e + 3]);
+                        send((chunk0 + c) * 128);
                     }
                 }
             }
@@ -794,22 +836,42 @@ CUresult encode_plane(CUtensorMap* map, const void* base, int n_kv, int num_bloc
                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
 }
 
-// One warp per (token, head) of the tiles' tokens: parts joined, normalised, stored.
+// Q as (128 channels, heads, tokens), boxes of 64 channels x the G heads of a KV head x
+// the tokens of 128 rows
+CUresult encode_q(CUtensorMap* map, const RowAttnParams& r, int n_tok) {
+    EncodeTiledFn enc = encode_tiled();
+    if (enc == nullptr) return CUDA_ERROR_NOT_SUPPORTED;
+    const cuuint64_t dim[3] = {PR_HD, (cuuint64_t)r.n_kv * r.G, (cuuint64_t)n_tok};
+    // (a dimension of one may come with any stride)
+    const cuuint64_t stride[2] = {(cuuint64_t)(r.n_kv * r.G > 1 ? r.q_head : PR_HD) * 2,
+                                  (cuuint64_t)(n_tok > 1 ? r.q_tok : PR_HD) * 2};
+    const cuuint32_t box[3] = {64, (cuuint32_t)r.G, (cuuint32_t)(TA_TILE / r.G)},
+                     one[3] = {1, 1, 1};
+    return enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<__nv_bfloat16*>(r.q), dim,
+               stride, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+}
+
+// One warp per (token, head) of the tiles' tokens: parts joined, normalised, stored.  (A
+// launch of its own: a warp that has eight parts' loads in flight and many warps to an SM;
+// at the end of the few-row kernel's CTAs the same reads took 5 us of each.)
 constexpr int TJ_WARPS = 8;
 __global__ void __launch_bounds__(32 * TJ_WARPS) join_parts_kernel(const TileAttnParams p,
-                                                                   int n_tok) {
+                                                                   int parts, int n_tok) {
     const int lane = threadIdx.x & 31, H = p.r.n_kv * p.r.G;
     const int64_t at = (int64_t)blockIdx.x * TJ_WARPS + (threadIdx.x >> 5);
     const int tok = (int)(at / H), h = (int)(at - (int64_t)tok * H);
     pdl_wait();
     if (tok >= n_tok || tok < p.bounds[0] || tok >= p.bounds[p.n_seg]) return;
-    int lo = 0, hi = p.n_seg - 1;                   // the token's request
-    while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (p.bounds[mid + 1] > tok) hi = mid; else lo = mid + 1;
+    if (!p.prefix_lens) {
+        int lo = 0, hi = p.n_seg - 1;               // the token's request
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (p.bounds[mid + 1] > tok) hi = mid; else lo = mid + 1;
+        }
+        if ((p.bounds[lo + 1] - p.bounds[lo]) * p.r.G <= p.min_rows) return;
     }
-    if ((p.bounds[lo + 1] - p.bounds[lo]) * p.r.G <= p.min_rows) return;
-    const PartSum s = join_parts(p.parts_out, p.parts_ml, p.part_rows, p.parts, at, 4 * lane);
+    const PartSum s = join_parts(p.parts_out, p.parts_ml, p.part_rows, parts, at, 4 * lane);
     const float inv = s.l > 0.f ? 1.f / s.l : 0.f;
     *reinterpret_cast<uint2*>(p.r.out + (int64_t)tok * p.r.o_tok + (int64_t)h * p.r.o_head +
                               4 * lane) =
@@ -821,11 +883,14 @@ __global__ void __launch_bounds__(32 * TJ_WARPS) join_parts_kernel(const TileAtt
 
 }  // namespace
 
-int launch_tile_attn(const char* who, TileAttnParams p, int max_tiles, cudaStream_t s) {
+int launch_tile_attn(const char* who, TileAttnParams p, int max_tiles, int n_tok,
+                     cudaStream_t s) {
     p.head_chunks = p.r.n_kv > 1 ? (int)(p.r.sh / 64) : 0;
     p.max_tiles = max_tiles;
-    CUtensorMap mk, mv;
-    CUresult cr = encode_plane(&mk, p.r.k, p.r.n_kv, p.r.num_blocks, 64 * p.head_chunks, p.r.st, p.r.sb);
+    CUtensorMap mq = {}, mk, mv;
+    CUresult cr = TA_TILE % p.r.G == 0 ? encode_q(&mq, p.r, n_tok) : CUDA_SUCCESS;
+    if (cr == CUDA_SUCCESS)
+        cr = encode_plane(&mk, p.r.k, p.r.n_kv, p.r.num_blocks, 64 * p.head_chunks, p.r.st, p.r.sb);
     if (cr == CUDA_SUCCESS)
         cr = encode_plane(&mv, p.r.v, p.r.n_kv, p.r.num_blocks, 64 * p.head_chunks, p.r.st,
                           p.r.sb);
@@ -843,11 +908,12 @@ int launch_tile_attn(const char* who, TileAttnParams p, int max_tiles, cudaStrea
     const int64_t items = (int64_t)max_tiles * p.r.n_kv * p.parts;
     LOCKS_REQUIRE(items < (1 << 30), LOCKS_ERR_SIZE, "%s: too many query rows in one call", who);
     tile_attn_kernel<<<(int)(items < sm_count() ? items : sm_count()), TA_THREADS, smem, s>>>(
-        mk, mv, p);
+        mq, mk, mv, p);
     return check_launch(who);
 }
 
-int launch_join_parts(const char* who, const TileAttnParams& p, int n_tok, cudaStream_t s) {
+int launch_join_parts(const char* who, const TileAttnParams& p, int parts, int n_tok,
+                      cudaStream_t s) {
     const int64_t rows = (int64_t)n_tok * p.r.n_kv * p.r.G;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)((rows + TJ_WARPS - 1) / TJ_WARPS), 1, 1);
@@ -858,7 +924,7 @@ int launch_join_parts(const char* who, const TileAttnParams& p, int n_tok, cudaS
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = pdl_enabled() ? 1 : 0;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, join_parts_kernel, p, n_tok);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, join_parts_kernel, p, parts, n_tok);
     if (e != cudaSuccess)
         return fail(LOCKS_ERR_LAUNCH, "%s: %s", who, cudaGetErrorString(e));
     return check_launch(who);

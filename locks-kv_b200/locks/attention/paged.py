@@ -106,7 +106,8 @@ def shared_prefix_paged_decode(q: torch.Tensor, kv_cache: torch.Tensor,
 
 
 def attention_scratch_floats(n_rows: int, n_heads: int, head_dim: int = 128,
-                             parts: int = 1) -> int:
+                             parts: int = 2) -> int:
     """fp32 elements that ``parts`` partial results of ``n_rows`` query tokens take
-    (a maximum, a sum and ``head_dim`` values per head)."""
+    (a maximum, a sum and ``head_dim`` values per head).  Shared-prefix decode needs
+    two, and uses up to one per 1 / (KV heads) of the device's SMs and one more."""
     return int(n_rows) * int(n_heads) * (int(head_dim) + 2) * int(parts)

@@ -349,7 +349,7 @@ PREFIX_CASES = [
 
 
 @pytest.mark.parametrize("case", range(len(PREFIX_CASES)))
-@pytest.mark.parametrize("more", [1, 7, 64])
+@pytest.mark.parametrize("more", [2, 7, 64])
 def test_prefix(case, more):
     n_kv, G, groups = PREFIX_CASES[case]
     g, cache, table, lens = prefix_paged(case, groups, n_kv)

@@ -86,7 +86,7 @@ def test_window_refusals(change, code, word):
 
 
 @pytest.mark.parametrize("change,code,word", SHARED + [
-    (dict(scratch=None), -1, "null"), (dict(pre=None), -1, "null"), (dict(floats=1039), -4, "1040"),
+    (dict(scratch=None), -1, "null"), (dict(pre=None), -1, "null"), (dict(floats=2079), -4, "2080"),
     (dict(n_groups=-1), -1, "size"), (dict(n_groups=0), 0, "")])
 def test_prefix_refusals(change, code, word):
     got, msg = rc("locks_shared_prefix_decode", with_(PREFIX, **change))
