@@ -97,7 +97,7 @@ _SIGNATURES = {
                                 _I, _I, _I, _I, _F, _P, _P], 1),
     "locks_shared_prefix_decode": ([_P, _L, _L, _P, _P, _L, _L, _L, _P, _L, _I, _I,
                                     _P, _P, _P, _P, _L, _L, _P, _L, _P, _L, _I, _I,
-                                    _I, _I, _I, _I, _F, _P, _P], 1),
+                                    _I, _I, _I, _I, _F, _P, _P], 3),
     "locks_mla_build_factors": ([_P, _L, _L, _P, _P, _I, _I, _P], 1),
     "locks_mla_refresh_rows": ([_P, _L, _L, _P, _P, _L, _P, _P, _P, _P, _P, _I, _I,
                                 _I, _P], 2),
@@ -111,6 +111,7 @@ _SIGNATURES = {
 }
 
 _lib = None
+_entries = {}         # bound entry points by name
 launches = 0          # kernels launched through this binding (bench evidence)
 
 
@@ -189,30 +190,45 @@ class CpLinkDesc(ctypes.Structure):
                 ("sink_loc", ctypes.c_int32), ("nsh_loc", ctypes.c_int32)]
 
 
-def call_on(dev: torch.device, name: str, *args) -> None:
-    """:func:`call` with ``dev`` current and its current stream as the last
-    argument (the tensors of a call need not live on the current device)."""
-    if dev.index == torch.cuda.current_device():
-        call(name, *args, c_void_p(torch.cuda.current_stream(dev).cuda_stream))
-        return
-    with torch.cuda.device(dev):
-        call(name, *args, c_void_p(torch.cuda.current_stream(dev).cuda_stream))
-
-
-def one_device(*tensors) -> torch.device:
-    """The CUDA device all of the tensors (None is passed over) live on."""
-    dev = None
+def one_device(*tensors) -> int:
+    """Index of the CUDA device all of the tensors (None is passed over) live on."""
+    dev = -1
     for t in tensors:
         if t is None:
             continue
-        if not t.is_cuda:
+        at = t.get_device()
+        if at < 0:
             raise RuntimeError("LOCKS B200 kernels need CUDA tensors, got "
                                f"{t.device}: there is no CPU path")
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
-            raise RuntimeError(f"tensors on {dev} and {t.device} in one call")
+        if dev < 0:
+            dev = at
+        elif at != dev:
+            raise RuntimeError(f"tensors on cuda:{dev} and cuda:{at} in one call")
     return dev
+
+
+def call_on(dev: int, name: str, *args) -> None:
+    """:func:`call` with device ``dev`` current and its current stream as the last
+    argument (the tensors of a call need not live on the current device); pointers
+    are passed as plain addresses."""
+    global launches
+    fn = _entries.get(name)
+    if fn is None:
+        fn = _entries[name] = getattr(lib(), name)
+    if dev == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    if rc != 0:
+        raise RuntimeError(
+            f"{name} failed ({rc}): {lib().locks_last_error().decode()}")
+    launches += _SIGNATURES[name][1]
+
+
+def addr(t):
+    """Address of a tensor whose device has been checked; None stays None."""
+    return None if t is None else t.data_ptr()
 
 
 def stream() -> c_void_p:

@@ -31,16 +31,18 @@ def append_plan(seq_lens: torch.Tensor, n_new: torch.Tensor,
     dev = _cabi.one_device(seq_lens, n_new, block_table, free_blocks, taken,
                            slot_mapping, positions, cu_tokens, lens_out, taken_out,
                            status)
-    R = seq_lens.shape[0]
+    i32, i64 = torch.int32, torch.int64
     for t in (seq_lens, n_new, free_blocks, taken, cu_tokens, lens_out, taken_out):
-        assert t.dtype == torch.int32 and t.is_contiguous(), \
+        assert t.dtype is i32 and t.is_contiguous(), \
             "lengths, counts and the free list are contiguous int32"
-    assert slot_mapping.dtype == positions.dtype == torch.int64
-    assert slot_mapping.is_contiguous() and positions.is_contiguous()
-    assert block_table.dtype == torch.int32 and block_table.stride(1) == 1
-    assert n_new.shape[0] == lens_out.shape[0] == block_table.shape[0] == R
-    assert cu_tokens.shape[0] == R + 1
-    assert positions.shape == slot_mapping.shape
+    assert slot_mapping.dtype is i64 and slot_mapping.is_contiguous()
+    assert positions.dtype is i64 and positions.is_contiguous()
+    R, cap = seq_lens.numel(), slot_mapping.numel()
+    rows, width = block_table.shape
+    stride = block_table.stride()
+    assert block_table.dtype is i32 and stride[1] == 1
+    assert n_new.numel() == lens_out.numel() == rows == R
+    assert cu_tokens.numel() == R + 1 and positions.numel() == cap
     assert taken.numel() == taken_out.numel() == 1
     if R == 0:
         cu_tokens.zero_()
@@ -49,10 +51,9 @@ def append_plan(seq_lens: torch.Tensor, n_new: torch.Tensor,
         if taken_out.data_ptr() != taken.data_ptr():
             taken_out.copy_(taken)
         return
-    _cabi.call_on(dev, "locks_append_plan", _cabi.ptr(seq_lens), _cabi.ptr(n_new),
-                  _cabi.ptr(block_table), max(block_table.stride(0), block_table.shape[1])
-                  if R == 1 else block_table.stride(0), block_table.shape[1],
-                  _cabi.ptr(free_blocks), free_blocks.shape[0], _cabi.ptr(taken),
-                  _cabi.ptr(slot_mapping), _cabi.ptr(positions), _cabi.ptr(cu_tokens),
-                  _cabi.ptr(lens_out), _cabi.ptr(taken_out), R, slot_mapping.shape[0],
-                  int(page), _cabi.ptr(status))
+    _cabi.call_on(dev, "locks_append_plan", seq_lens.data_ptr(), n_new.data_ptr(),
+                  block_table.data_ptr(), width if R == 1 else stride[0], width,
+                  free_blocks.data_ptr(), free_blocks.numel(), taken.data_ptr(),
+                  slot_mapping.data_ptr(), positions.data_ptr(), cu_tokens.data_ptr(),
+                  lens_out.data_ptr(), taken_out.data_ptr(), R, cap, page,
+                  _cabi.addr(status))

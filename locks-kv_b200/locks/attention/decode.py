@@ -39,6 +39,19 @@ def _split_kv(kv_cache: torch.Tensor):
     return kv_cache.select(1, 0), kv_cache.select(1, 1)
 
 
+def _planes(kv_cache: torch.Tensor):
+    """Addresses of the K and V planes of a cache in either layout of
+    :func:`_split_kv`, their (blocks, page, n_kv, d) and their strides."""
+    shape, stride = kv_cache.shape, kv_cache.stride()
+    k = kv_cache.data_ptr()
+    if shape[0] == 2:
+        return (k, k + stride[0] * kv_cache.element_size(), shape[1:],
+                stride[1:])
+    assert shape[1] == 2, "the cache has no V half"
+    return (k, k + stride[1] * kv_cache.element_size(), (shape[0], *shape[2:]),
+            (stride[0], *stride[2:]))
+
+
 class ResidentVSource:
     """V lives in the engine cache next to K (the ``fast`` variant)."""
     SRC_ID = 0

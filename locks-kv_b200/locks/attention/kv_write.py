@@ -15,7 +15,7 @@ from typing import Optional
 import torch
 
 from .. import _cabi
-from .decode import _split_kv
+from .decode import _planes, _split_kv
 
 
 def rope_and_cache(key: torch.Tensor, val: torch.Tensor, kv_cache: torch.Tensor,
@@ -108,41 +108,42 @@ def norm_rope_and_cache(q: torch.Tensor, key: torch.Tensor, val: torch.Tensor,
     beyond the cache) stores nothing.  Returns ``q_out``."""
     if q_out is None:
         q_out = q
-    k, v = _split_kv(kv_cache)
-    assert v is not None, "the cache has no V half"
     dev = _cabi.one_device(q, key, val, kv_cache, slot_mapping, positions, cos_sin,
                            q_weight, k_weight, q_out)
-    bf16, f32 = torch.bfloat16, torch.float32
-    assert q.dtype == key.dtype == val.dtype == q_out.dtype == k.dtype == bf16
-    assert q.stride(2) == key.stride(2) == val.stride(2) == q_out.stride(2) == 1
-    assert k.stride(3) == 1 and v.stride(3) == 1
-    assert k.stride() == v.stride(), "K and V planes must share strides"
-    n_tok, H, d = q.shape
-    n_kv = key.shape[1]
-    assert key.shape == val.shape == (n_tok, n_kv, d) and q_out.shape == q.shape
-    assert k.shape[2] == n_kv and k.shape[3] == d
-    assert slot_mapping.dtype == torch.int64 and slot_mapping.is_contiguous()
-    assert slot_mapping.shape[0] >= n_tok
-    rot = rows = stride = t_f32 = 0
+    k, v, (n_blocks, page, n_kv, d), cs = _planes(kv_cache)
+    bf16, f32, i64 = torch.bfloat16, torch.float32, torch.int64
+    assert q.dtype is bf16 and key.dtype is bf16 and val.dtype is bf16
+    assert q_out.dtype is bf16 and kv_cache.dtype is bf16
+    n_tok, H, _ = shape = q.shape
+    assert q_out.shape == shape and shape[2] == d
+    assert key.shape == val.shape == (n_tok, n_kv, d)
+    qs, ks, vs, os = q.stride(), key.stride(), val.stride(), q_out.stride()
+    assert qs[2] == ks[2] == vs[2] == os[2] == cs[3] == 1
+    assert slot_mapping.dtype is i64 and slot_mapping.is_contiguous()
+    assert slot_mapping.numel() >= n_tok
+    rot = rows = row_stride = t_f32 = 0
     if cos_sin is not None:
-        assert positions is not None and positions.dtype == torch.int64
-        assert positions.is_contiguous() and positions.shape[0] >= n_tok
-        assert cos_sin.dtype in (bf16, f32) and cos_sin.stride(1) == 1
+        assert positions is not None and positions.dtype is i64
+        assert positions.is_contiguous() and positions.numel() >= n_tok
+        t_f32 = cos_sin.dtype is f32
         rows, rot = cos_sin.shape
-        stride = max(cos_sin.stride(0), rot) if rows == 1 else cos_sin.stride(0)
-        t_f32 = int(cos_sin.dtype == f32)
-    weights = [w for w in (q_weight, k_weight) if w is not None]
-    for w in weights:
-        assert w.dtype in (bf16, f32) and w.dtype == weights[0].dtype, \
-            "norm weights are bf16 or fp32, both alike"
-        assert w.shape == (d,) and w.is_contiguous()
-    _cabi.call_on(dev, "locks_norm_rope_write", _cabi.ptr(q), q.stride(0), q.stride(1),
-                  _cabi.ptr(key), key.stride(0), key.stride(1), _cabi.ptr(val),
-                  val.stride(0), val.stride(1), _cabi.ptr(q_out), q_out.stride(0),
-                  q_out.stride(1), _cabi.ptr(k), _cabi.ptr(v), k.stride(0), k.stride(1),
-                  k.stride(2), _cabi.ptr(slot_mapping), _cabi.ptr(positions),
-                  _cabi.ptr(cos_sin), stride, rows, rot, int(neox), t_f32,
-                  _cabi.ptr(q_weight), _cabi.ptr(k_weight),
-                  int(bool(weights) and weights[0].dtype == f32), float(eps), n_tok, H,
-                  n_kv, d, k.shape[1], k.shape[0])
+        row_stride, one = cos_sin.stride()
+        assert one == 1 and (t_f32 or cos_sin.dtype is bf16)
+        if rows == 1:
+            row_stride = rot
+    w_f32 = 0
+    if q_weight is not None or k_weight is not None:
+        some = q_weight if q_weight is not None else k_weight
+        w_f32 = some.dtype is f32
+        for w in (q_weight, k_weight):
+            assert w is None or (w.dtype is some.dtype and w.numel() == d and
+                                 w.is_contiguous()), \
+                "norm weights are contiguous (d,) tensors of one type"
+        assert w_f32 or some.dtype is bf16, "norm weights are bf16 or fp32"
+    _cabi.call_on(dev, "locks_norm_rope_write", q.data_ptr(), qs[0], qs[1],
+                  key.data_ptr(), ks[0], ks[1], val.data_ptr(), vs[0], vs[1],
+                  q_out.data_ptr(), os[0], os[1], k, v, cs[0], cs[1], cs[2],
+                  slot_mapping.data_ptr(), _cabi.addr(positions), _cabi.addr(cos_sin),
+                  row_stride, rows, rot, neox, t_f32, _cabi.addr(q_weight),
+                  _cabi.addr(k_weight), w_f32, eps, n_tok, H, n_kv, d, page, n_blocks)
     return q_out

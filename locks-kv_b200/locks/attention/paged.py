@@ -8,35 +8,37 @@ from typing import Optional
 import torch
 
 from .. import _cabi
-from .decode import _split_kv
+from .decode import _planes
 
 NO_WINDOW = 2 ** 31 - 1
 
 
-def _checked(q, kv_cache, block_table, out, lse, n_kv, G, ints):
-    k, v = _split_kv(kv_cache)
-    assert v is not None, "the cache has no V half"
-    bf16 = torch.bfloat16
-    assert q.dtype == out.dtype == k.dtype == bf16
-    assert q.dim() == 3 and q.shape[1] == n_kv * G and out.shape == q.shape
-    assert q.stride(2) == out.stride(2) == k.stride(3) == v.stride(3) == 1
-    assert k.stride() == v.stride(), "K and V planes must share strides"
-    assert k.shape[2] == n_kv and k.shape[3] == q.shape[2]
-    assert block_table.dtype == torch.int32 and block_table.stride(1) == 1
+def _checked(q, kv_cache, block_table, out, lse, scratch, n_kv, G, ints):
+    """What both calls check of their tensors; the arguments both pass on."""
+    k, v, (n_blocks, page, heads, d), cs = _planes(kv_cache)
+    bf16, f32, i32 = torch.bfloat16, torch.float32, torch.int32
+    assert q.dtype is bf16 and out.dtype is bf16 and kv_cache.dtype is bf16
+    shape, qs, os = q.shape, q.stride(), out.stride()
+    assert len(shape) == 3 and out.shape == shape
+    assert shape[1] == n_kv * G and heads == n_kv and shape[2] == d
+    assert qs[2] == os[2] == cs[3] == 1
+    bs = block_table.stride()
+    assert block_table.dtype is i32 and bs[1] == 1
     for t in ints:
-        assert t.dtype == torch.int32 and t.is_contiguous(), \
+        assert t.dtype is i32 and t.is_contiguous(), \
             "lengths and bounds are contiguous int32"
+    lse_at, lse_stride, scratch_at, floats = None, 0, None, 0
     if lse is not None:
-        assert lse.dtype == torch.float32 and lse.stride(1) == 1
-        assert lse.shape == q.shape[:2]
-    return k, v
-
-
-def _scratch(scratch):
-    if scratch is None:
-        return 0
-    assert scratch.dtype == torch.float32 and scratch.is_contiguous()
-    return scratch.numel()
+        lse_stride, one = lse.stride()
+        assert lse.dtype is f32 and one == 1 and lse.shape == shape[:2]
+        lse_at = lse.data_ptr()
+    if scratch is not None:
+        assert scratch.dtype is f32 and scratch.is_contiguous()
+        scratch_at, floats = scratch.data_ptr(), scratch.numel()
+    return ((q.data_ptr(), qs[0], qs[1], k, v, cs[0], cs[1], cs[2],
+             block_table.data_ptr(), bs[0], block_table.shape[1], n_blocks),
+            (out.data_ptr(), os[0], os[1], lse_at, lse_stride, scratch_at, floats),
+            d, page)
 
 
 def window_paged_attention(q: torch.Tensor, kv_cache: torch.Tensor,
@@ -57,21 +59,16 @@ def window_paged_attention(q: torch.Tensor, kv_cache: torch.Tensor,
     ``max_q`` bounds the query tokens of a request.  ``scratch``: fp32 workspace
     for long keys with few queries, see :func:`attention_scratch_floats`; calls
     that may overlap on the GPU need one each."""
-    k, v = _checked(q, kv_cache, block_table, out, lse, n_kv, G, (cu_q, seq_lens))
     dev = _cabi.one_device(q, kv_cache, block_table, cu_q, seq_lens, out, scratch, lse,
                            status)
-    R = seq_lens.shape[0]
-    assert cu_q.shape[0] == R + 1 and block_table.shape[0] == R
-    _cabi.call_on(dev, "locks_window_attention", _cabi.ptr(q), q.stride(0), q.stride(1),
-                  _cabi.ptr(k), _cabi.ptr(v), k.stride(0), k.stride(1), k.stride(2),
-                  _cabi.ptr(block_table), block_table.stride(0), block_table.shape[1],
-                  k.shape[0], _cabi.ptr(cu_q), _cabi.ptr(seq_lens), _cabi.ptr(out),
-                  out.stride(0), out.stride(1), _cabi.ptr(lse),
-                  lse.stride(0) if lse is not None else 0, _cabi.ptr(scratch),
-                  _scratch(scratch), q.shape[0], R, int(max_q), int(n_kv), int(G),
-                  q.shape[2], k.shape[1],
-                  NO_WINDOW if window is None else min(int(window), NO_WINDOW),
-                  int(sinks), float(scale), _cabi.ptr(status))
+    source, target, d, page = _checked(q, kv_cache, block_table, out, lse, scratch,
+                                       n_kv, G, (cu_q, seq_lens))
+    R = seq_lens.numel()
+    assert cu_q.numel() == R + 1 and block_table.shape[0] == R
+    _cabi.call_on(dev, "locks_window_attention", *source, cu_q.data_ptr(),
+                  seq_lens.data_ptr(), *target, q.shape[0], R, max_q, n_kv, G, d, page,
+                  NO_WINDOW if window is None else min(window, NO_WINDOW), sinks,
+                  scale, _cabi.addr(status))
 
 
 def shared_prefix_paged_decode(q: torch.Tensor, kv_cache: torch.Tensor,
@@ -87,22 +84,16 @@ def shared_prefix_paged_decode(q: torch.Tensor, kv_cache: torch.Tensor,
     (through the table row of its first request).  Writes ``out`` (and ``lse``) in
     place; rows outside the groups stay as they were.  ``scratch``: fp32 workspace,
     at least ``attention_scratch_floats(R, H, d)`` elements."""
-    k, v = _checked(q, kv_cache, block_table, out, lse, n_kv, G,
-                    (seq_lens, cu_groups, prefix_lens))
     dev = _cabi.one_device(q, kv_cache, block_table, seq_lens, cu_groups, prefix_lens,
                            out, scratch, lse, status)
-    R = q.shape[0]
-    assert seq_lens.shape[0] == block_table.shape[0] == R
-    assert cu_groups.shape[0] == prefix_lens.shape[0] + 1
-    _cabi.call_on(dev, "locks_shared_prefix_decode", _cabi.ptr(q), q.stride(0),
-                  q.stride(1), _cabi.ptr(k), _cabi.ptr(v), k.stride(0), k.stride(1),
-                  k.stride(2), _cabi.ptr(block_table), block_table.stride(0),
-                  block_table.shape[1], k.shape[0], _cabi.ptr(seq_lens),
-                  _cabi.ptr(cu_groups), _cabi.ptr(prefix_lens), _cabi.ptr(out),
-                  out.stride(0), out.stride(1), _cabi.ptr(lse),
-                  lse.stride(0) if lse is not None else 0, _cabi.ptr(scratch),
-                  _scratch(scratch), R, prefix_lens.shape[0], int(n_kv), int(G),
-                  q.shape[2], k.shape[1], float(scale), _cabi.ptr(status))
+    source, target, d, page = _checked(q, kv_cache, block_table, out, lse, scratch,
+                                       n_kv, G, (seq_lens, cu_groups, prefix_lens))
+    R, groups = q.shape[0], prefix_lens.numel()
+    assert seq_lens.numel() == block_table.shape[0] == R
+    assert cu_groups.numel() == groups + 1
+    _cabi.call_on(dev, "locks_shared_prefix_decode", *source, seq_lens.data_ptr(),
+                  cu_groups.data_ptr(), prefix_lens.data_ptr(), *target, R, groups,
+                  n_kv, G, d, page, scale, _cabi.addr(status))
 
 
 def attention_scratch_floats(n_rows: int, n_heads: int, head_dim: int = 128,
