@@ -30,10 +30,10 @@ namespace cg = cooperative_groups;
 namespace locks {
 namespace {
 
-constexpr int AP_THREADS = 512;
+constexpr int AP_THREADS = 1024;
 constexpr int AP_WARPS = AP_THREADS / 32;
 constexpr int AP_MAX_REQS = 4096;
-constexpr int AP_MAX_CL = 8;
+constexpr int AP_MAX_CL = 16;
 
 struct PlanParams {
     const int32_t* seq_lens;
@@ -202,6 +202,8 @@ extern "C" int locks_append_plan(const int32_t* seq_lens, const int32_t* n_new,
         cudaFuncSetAttribute(append_plan_kernel,
                              cudaFuncAttributeMaxDynamicSharedMemorySize,
                              (3 * AP_MAX_REQS + 1) * (int)sizeof(int));
+        cudaFuncSetAttribute(append_plan_kernel,
+                             cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         attr_done[dev] = true;
     }
     int cl = 1;

@@ -9,9 +9,9 @@
 //
 // Bound by memory: a row is read and written once, 2 * 256 B.  A half-warp owns a
 // row (16 lanes x 8 channels = one 16-byte access per lane), so the norm is four
-// shuffles and the half-split partner sits half/8 lanes away; rows of a token are
-// neighbours, so its (cos | sin) row comes from L1 after the first.  A half-warp
-// takes NR_ROWS rows and has all their loads in flight before the first is used.
+// shuffles and the half-split partner sits half/8 lanes away.  A warp takes NR_ROWS
+// pairs of neighbouring rows of one token: their loads are all in flight before the
+// first is used, and the token's slot, position and (cos | sin) row are read once.
 #include "common.cuh"
 
 namespace locks {
@@ -36,7 +36,7 @@ struct NormRopeParams {
     int64_t cs_row;
     const void *q_weight, *k_weight;
     int weight_f32, rot, neox, n_pos, num_blocks;
-    int n_tok, H, n_kv;
+    int n_tok, H, n_kv, chunks;                    // chunks of 2 NR_ROWS heads a token
     float eps;
 };
 
@@ -79,120 +79,115 @@ __device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162flo
 template <int MODE, class Tab>
 __global__ void __launch_bounds__(NR_THREADS) norm_rope_kernel(const NormRopeParams p) {
     __shared__ float stage[MODE == ROPE_ANY ? NR_HALVES : 1][MODE == ROPE_ANY ? NR_HD : 1];
-    const int half_id = threadIdx.x >> 4, lane = threadIdx.x & 15;
+    const int half_id = threadIdx.x >> 4, lane = threadIdx.x & 15, side = half_id & 1;
     const int heads = p.H + 2 * p.n_kv;
-    const int64_t n_rows = (int64_t)p.n_tok * heads;
-    const int64_t row0 = (int64_t)blockIdx.x * (NR_HALVES * NR_ROWS) + half_id;
+    const int unit = blockIdx.x * (NR_THREADS / 32) + (threadIdx.x >> 5);
+    const int t = unit / p.chunks;
+    if (t >= p.n_tok) return;                    // (a whole warp)
+    const int h0 = (unit - t * p.chunks) * (2 * NR_ROWS) + side;
 
     uint4 x[NR_ROWS];
-    int tok[NR_ROWS], head[NR_ROWS];
-    int64_t slot[NR_ROWS];
 #pragma unroll
     for (int i = 0; i < NR_ROWS; ++i) {
-        const int64_t row = row0 + i * NR_HALVES;
-        tok[i] = -1;
-        slot[i] = 0;
+        const int h = h0 + 2 * i;
         x[i] = make_uint4(0, 0, 0, 0);
-        if (row >= n_rows) continue;
-        const int t = (int)(row / heads), h = (int)(row - (int64_t)t * heads);
-        tok[i] = t;
-        head[i] = h;
+        if (h >= heads) continue;
         const __nv_bfloat16* src =
             h < p.H ? p.q + t * p.q_tok + h * p.q_head
             : h < p.H + p.n_kv ? p.k + t * p.k_tok + (h - p.H) * p.k_head
                                : p.v + t * p.v_tok + (h - p.H - p.n_kv) * p.v_head;
         x[i] = *reinterpret_cast<const uint4*>(src + 8 * lane);
-        if (h >= p.H) slot[i] = p.slot[t];
     }
+    const int64_t slot = p.slot[t];
+    // the token's table row, as far as this lane's channels need it
+    const int half = p.rot >> 1;
+    const Tab* cs = static_cast<const Tab*>(p.cos_sin);
+    const bool turns = 8 * lane < p.rot;
+    const int hl = half >> 3;                    // half-split: lanes of one half
+    const bool low = lane < hl;
+    float c[8], s[8];
+    if constexpr (MODE != ROPE_NONE) {
+        cs += min(max(p.pos[t], (int64_t)0), (int64_t)p.n_pos - 1) * p.cs_row;
+        if (MODE == ROPE_PAIRS && turns) {       // rot a multiple of 8
+            float (&c4)[4] = reinterpret_cast<float (&)[4]>(c);
+            float (&s4)[4] = reinterpret_cast<float (&)[4]>(s);
+            load_vals(cs + 4 * lane, c4);
+            load_vals(cs + half + 4 * lane, s4);
+        }
+        if (MODE == ROPE_HALVES && turns) {      // half a multiple of 8
+            const int d = 8 * (low ? lane : lane - hl);
+            load_vals(cs + d, c);
+            load_vals(cs + half + d, s);
+        }
+    }
+    const bool stored = slot >= 0 && (slot >> 4) < p.num_blocks;
+    const int64_t at = stored ? (slot >> 4) * p.cb + (slot & 15) * p.ct : 0;
 #pragma unroll
     for (int i = 0; i < NR_ROWS; ++i) {
         // (both half-warps of a warp run every round: the shuffles need all lanes)
-        const int t = max(tok[i], 0), h = tok[i] < 0 ? 0 : head[i];
+        const int h = h0 + 2 * i;
         const bool is_q = h < p.H, is_k = !is_q && h < p.H + p.n_kv;
         uint4 y = x[i];
         float f[8];
         unpack8(x[i], f);
         const void* wt = is_q ? p.q_weight : is_k ? p.k_weight : nullptr;
-        {
-            float ss = 0.f;
+        float ss = 0.f;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) ss += f[e] * f[e];
+        for (int e = 0; e < 8; ++e) ss += f[e] * f[e];
 #pragma unroll
-            for (int d = 1; d < 16; d <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
-            if (wt) {
-                const float rs = rsqrtf(ss * (1.f / NR_HD) + p.eps);
-                float w[8];
-                if (p.weight_f32) load_vals(static_cast<const float*>(wt) + 8 * lane, w);
-                else load_vals(static_cast<const __nv_bfloat16*>(wt) + 8 * lane, w);
+        for (int d = 1; d < 16; d <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
+        if (wt) {
+            const float rs = rsqrtf(ss * (1.f / NR_HD) + p.eps);
+            float w[8];
+            if (p.weight_f32) load_vals(static_cast<const float*>(wt) + 8 * lane, w);
+            else load_vals(static_cast<const __nv_bfloat16*>(wt) + 8 * lane, w);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) f[e] = f[e] * rs * w[e];
-            }
+            for (int e = 0; e < 8; ++e) f[e] = f[e] * rs * w[e];
         }
-        if constexpr (MODE != ROPE_NONE) {
-            int64_t at = 0;
-            if (is_q || is_k) at = min(max(p.pos[t], (int64_t)0), (int64_t)p.n_pos - 1);
-            const Tab* cs = static_cast<const Tab*>(p.cos_sin) + at * p.cs_row;
-            const int half = p.rot >> 1;
-            const bool turns = (is_q || is_k) && 8 * lane < p.rot;
-            if constexpr (MODE == ROPE_PAIRS) {             // rot a multiple of 8
-                if (turns) {
-                    float c[4], s[4];
-                    load_vals(cs + 4 * lane, c);
-                    load_vals(cs + half + 4 * lane, s);
+        if constexpr (MODE == ROPE_PAIRS) {
+            if (turns) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float a = f[2 * e], b = f[2 * e + 1];
-                        f[2 * e] = a * c[e] - b * s[e];
-                        f[2 * e + 1] = b * c[e] + a * s[e];
-                    }
+                for (int e = 0; e < 4; ++e) {
+                    const float a = f[2 * e], b = f[2 * e + 1];
+                    f[2 * e] = a * c[e] - b * s[e];
+                    f[2 * e + 1] = b * c[e] + a * s[e];
                 }
-            } else if constexpr (MODE == ROPE_HALVES) {     // half a multiple of 8
-                const int hl = half >> 3;                   // lanes of one half
-                const bool low = lane < hl;
-                const int partner = low ? lane + hl : lane - hl;
-                float o[8];
+            }
+        } else if constexpr (MODE == ROPE_HALVES) {
+            const int partner = turns ? (low ? lane + hl : lane - hl) : lane;
+            float o[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) o[e] = __shfl_sync(0xffffffffu, f[e], partner, 16);
+            if (turns) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
-                    o[e] = __shfl_sync(0xffffffffu, f[e], turns ? partner : lane, 16);
-                if (turns) {
-                    float c[8], s[8];
-                    const int d = 8 * (low ? lane : lane - hl);
-                    load_vals(cs + d, c);
-                    load_vals(cs + half + d, s);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        f[e] = low ? f[e] * c[e] - o[e] * s[e] : f[e] * c[e] + o[e] * s[e];
-                }
-            } else {                                        // any even rot, any alignment
-#pragma unroll
-                for (int e = 0; e < 8; ++e) stage[half_id][8 * lane + e] = f[e];
-                __syncwarp();
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const int d = 8 * lane + e;
-                    if ((is_q || is_k) && d < p.rot) {
-                        const bool low = p.neox ? d < half : (d & 1) == 0;
-                        const int o = p.neox ? (low ? d + half : d - half) : d ^ 1;
-                        const int j = p.neox ? (low ? d : d - half) : d >> 1;
-                        const float c = to_f32(cs[j]), s = to_f32(cs[half + j]);
-                        f[e] = low ? f[e] * c - stage[half_id][o] * s
-                                   : f[e] * c + stage[half_id][o] * s;
-                    }
-                }
-                __syncwarp();
+                    f[e] = low ? f[e] * c[e] - o[e] * s[e] : f[e] * c[e] + o[e] * s[e];
             }
+        } else if constexpr (MODE == ROPE_ANY) {            // any even rot, any alignment
+#pragma unroll
+            for (int e = 0; e < 8; ++e) stage[half_id][8 * lane + e] = f[e];
+            __syncwarp();
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int d = 8 * lane + e;
+                if ((is_q || is_k) && d < p.rot) {
+                    const bool first = p.neox ? d < half : (d & 1) == 0;
+                    const int o = p.neox ? (first ? d + half : d - half) : d ^ 1;
+                    const int j = p.neox ? (first ? d : d - half) : d >> 1;
+                    const float cj = to_f32(cs[j]), sj = to_f32(cs[half + j]);
+                    f[e] = first ? f[e] * cj - stage[half_id][o] * sj
+                                 : f[e] * cj + stage[half_id][o] * sj;
+                }
+            }
+            __syncwarp();
         }
         if (is_q || is_k) y = pack8(f);
-        if (tok[i] < 0) continue;
         if (is_q) {
             *reinterpret_cast<uint4*>(p.q_out + t * p.o_tok + h * p.o_head + 8 * lane) = y;
-        } else {
-            const int64_t blk = slot[i] >> 4;
-            if (slot[i] >= 0 && blk < p.num_blocks) {
-                const int kh = is_k ? h - p.H : h - p.H - p.n_kv;
-                *reinterpret_cast<uint4*>((is_k ? p.k_cache : p.v_cache) + blk * p.cb +
-                                          (slot[i] & 15) * p.ct + kh * p.ch + 8 * lane) = y;
-            }
+        } else if (h < heads && stored) {
+            const int kh = is_k ? h - p.H : h - p.H - p.n_kv;
+            *reinterpret_cast<uint4*>((is_k ? p.k_cache : p.v_cache) + at + kh * p.ch +
+                                      8 * lane) = y;
         }
     }
 }
@@ -232,7 +227,7 @@ extern "C" int locks_norm_rope_write(
                   "locks_norm_rope_write: supports head_dim 128 / page 16, got %d / %d",
                   head_dim, page);
     LOCKS_REQUIRE(n_tok >= 0 && n_heads >= 1 && n_kv >= 1 && num_blocks >= 1 &&
-                      (int64_t)n_tok * (n_heads + 2 * n_kv) <= (int64_t)1 << 36,
+                      (int64_t)n_tok * (n_heads + 2 * n_kv) < (int64_t)1 << 31,
                   LOCKS_ERR_ARG, "locks_norm_rope_write: bad size argument");
     LOCKS_REQUIRE(rows16(q, q_stride_tok, q_stride_head) &&
                       rows16(key, k_stride_tok, k_stride_head) &&
@@ -284,9 +279,9 @@ extern "C" int locks_norm_rope_write(
                : neox ? (half % 8 == 0 ? ROPE_HALVES : ROPE_ANY)
                       : (rot_dim % 8 == 0 ? ROPE_PAIRS : ROPE_ANY);
     }
-    const int64_t rows = (int64_t)n_tok * (n_heads + 2 * n_kv);
-    const int64_t per = NR_HALVES * NR_ROWS;
-    const dim3 grid((unsigned)((rows + per - 1) / per), 1, 1);
+    p.chunks = (n_heads + 2 * n_kv + 2 * NR_ROWS - 1) / (2 * NR_ROWS);
+    constexpr int WARPS = NR_THREADS / 32;
+    const dim3 grid((unsigned)(((int64_t)n_tok * p.chunks + WARPS - 1) / WARPS), 1, 1);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (table_f32) launch_norm_rope<float>(mode, grid, s, p);
     else launch_norm_rope<__nv_bfloat16>(mode, grid, s, p);
