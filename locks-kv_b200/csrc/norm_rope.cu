@@ -8,8 +8,9 @@
 // All of it in fp32 with one rounding to bf16 at the end.
 //
 // Bound by memory: a row is read and written once, 2 * 256 B.  A half-warp owns a
-// row (16 lanes x 8 channels = one 16-byte access per lane), so the norm is four
-// shuffles and the half-split partner sits half/8 lanes away.  A warp takes one token
+// row, 16 lanes x 8 channels, so the norm is four shuffles.  A lane's channels are eight
+// in a row (one 16-byte access), or in half-split pairing four of each half (two of 8
+// bytes), so that both channels of a pair are its own.  A warp takes one token
 // (or, where there are few tokens, a share of its heads), whose slot, position and
 // (cos | sin) row it reads once, in steps of NR_ROWS pairs of neighbouring rows; the
 // next step's rows are on their way while a step is computed.  Pairs of channels share
@@ -94,9 +95,32 @@ __global__ void __launch_bounds__(NR_THREADS, 8) norm_rope_kernel(const NormRope
     if (t >= p.n_tok) return;                    // (a whole warp)
     int h0 = (job - t * p.shares) * p.share;     // the warp's heads [h0, end)
     const int end = min(h0 + p.share, heads);
-    const __nv_bfloat16* q = p.q + t * p.q_tok + 8 * lane;
-    const __nv_bfloat16* k = p.k + t * p.k_tok + 8 * lane;
-    const __nv_bfloat16* v = p.v + t * p.v_tok + 8 * lane;
+    // the lane's channels: [ca, ca + 4) and [cb, cb + 4).  Half-split: of either half
+    // while there are rotated ones, the rest in order
+    const int half = p.rot >> 1, quads = half >> 2;
+    const bool turns = MODE == ROPE_HALVES ? lane < quads : 8 * lane < p.rot;
+    const int ca = MODE != ROPE_HALVES ? 8 * lane : turns ? 4 * lane : p.rot + 8 * (lane - quads);
+    const int cb = MODE == ROPE_HALVES && turns ? ca + half : ca + 4;
+    auto load_row = [&](const __nv_bfloat16* row) {
+        if constexpr (MODE == ROPE_HALVES) {
+            const uint2 a = *reinterpret_cast<const uint2*>(row + ca);
+            const uint2 b = *reinterpret_cast<const uint2*>(row + cb);
+            return make_uint4(a.x, a.y, b.x, b.y);
+        } else {
+            return *reinterpret_cast<const uint4*>(row + ca);
+        }
+    };
+    auto store_row = [&](__nv_bfloat16* row, const uint4 y) {
+        if constexpr (MODE == ROPE_HALVES) {
+            *reinterpret_cast<uint2*>(row + ca) = make_uint2(y.x, y.y);
+            *reinterpret_cast<uint2*>(row + cb) = make_uint2(y.z, y.w);
+        } else {
+            *reinterpret_cast<uint4*>(row + ca) = y;
+        }
+    };
+    const __nv_bfloat16* q = p.q + t * p.q_tok;
+    const __nv_bfloat16* k = p.k + t * p.k_tok;
+    const __nv_bfloat16* v = p.v + t * p.v_tok;
 
     uint4 next[NR_ROWS];
     auto fetch = [&](int first) {
@@ -107,7 +131,7 @@ __global__ void __launch_bounds__(NR_THREADS, 8) norm_rope_kernel(const NormRope
             const __nv_bfloat16* src = h < p.H ? q + h * p.q_head
                                        : h < qk ? k + (h - p.H) * p.k_head
                                                 : v + (h - qk) * p.v_head;
-            next[i] = *reinterpret_cast<const uint4*>(src);
+            next[i] = load_row(src);
         }
     };
 #pragma unroll
@@ -115,27 +139,15 @@ __global__ void __launch_bounds__(NR_THREADS, 8) norm_rope_kernel(const NormRope
     fetch(h0);
     const int64_t slot = p.slot[t];
     // the token's table row, as far as this lane's channels need it
-    const int half = p.rot >> 1;
     const Tab* cs = static_cast<const Tab*>(p.cos_sin);
-    const bool turns = 8 * lane < p.rot;
-    const int hl = half >> 3;                    // half-split: lanes of one half
-    const bool low = lane < hl;
     float2 c[4], s[4];
     if constexpr (MODE != ROPE_NONE) {
         cs += min(max(p.pos[t], (int64_t)0), (int64_t)p.n_pos - 1) * p.cs_row;
-        if (MODE == ROPE_PAIRS && turns) {       // rot a multiple of 8
+        if ((MODE == ROPE_PAIRS || MODE == ROPE_HALVES) && turns) {
             float2 (&c2)[2] = reinterpret_cast<float2 (&)[2]>(c);
             float2 (&s2)[2] = reinterpret_cast<float2 (&)[2]>(s);
             load_vals(cs + 4 * lane, c2);
             load_vals(cs + half + 4 * lane, s2);
-        }
-        if (MODE == ROPE_HALVES && turns) {      // half a multiple of 8
-            const int d = 8 * (low ? lane : lane - hl);
-            load_vals(cs + d, c);
-            load_vals(cs + half + d, s);
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (low) s[e] = make_float2(-s[e].x, -s[e].y);
         }
         if (MODE == ROPE_ANY) {                  // any even rot, any alignment
 #pragma unroll
@@ -153,7 +165,7 @@ __global__ void __launch_bounds__(NR_THREADS, 8) norm_rope_kernel(const NormRope
         }
     }
     const bool stored = slot >= 0 && (slot >> 4) < p.num_blocks;
-    const int64_t at = stored ? (slot >> 4) * p.cb + (slot & 15) * p.ct + 8 * lane : 0;
+    const int64_t at = stored ? (slot >> 4) * p.cb + (slot & 15) * p.ct : 0;
     for (; h0 < end; h0 += 2 * NR_ROWS) {
         uint4 x[NR_ROWS];
 #pragma unroll
@@ -179,12 +191,15 @@ __global__ void __launch_bounds__(NR_THREADS, 8) norm_rope_kernel(const NormRope
                 for (int d = 1; d < 16; d <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
                 if (wt) {
                     const float rs = rsqrtf(ss * (1.f / NR_HD) + p.eps);
-                    float2 w[4];
-                    if (p.weight_f32) load_vals(static_cast<const float*>(wt) + 8 * lane, w);
-                    else load_vals(static_cast<const __nv_bfloat16*>(wt) + 8 * lane, w);
+                    float2 w[2];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        f[e] = nr_mul2(nr_mul2(f[e], make_float2(rs, rs)), w[e]);
+                    for (int e = 0; e < 4; e += 2) {
+                        const int ch = e ? cb : ca;
+                        if (p.weight_f32) load_vals(static_cast<const float*>(wt) + ch, w);
+                        else load_vals(static_cast<const __nv_bfloat16*>(wt) + ch, w);
+                        f[e] = nr_mul2(nr_mul2(f[e], make_float2(rs, rs)), w[0]);
+                        f[e + 1] = nr_mul2(nr_mul2(f[e + 1], make_float2(rs, rs)), w[1]);
+                    }
                 }
                 if constexpr (MODE == ROPE_PAIRS) {
                     if (turns) {
@@ -197,15 +212,13 @@ __global__ void __launch_bounds__(NR_THREADS, 8) norm_rope_kernel(const NormRope
                         }
                     }
                 } else if constexpr (MODE == ROPE_HALVES) {
-                    const int partner = turns ? (low ? lane + hl : lane - hl) : lane;
-                    float2 o[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        o[e] = make_float2(__shfl_sync(0xffffffffu, f[e].x, partner, 16),
-                                           __shfl_sync(0xffffffffu, f[e].y, partner, 16));
                     if (turns) {
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) f[e] = nr_fma2(o[e], s[e], nr_mul2(f[e], c[e]));
+                        for (int e = 0; e < 2; ++e) {
+                            const float2 a = f[e], b = f[2 + e];
+                            f[e] = nr_fma2(b, make_float2(-s[e].x, -s[e].y), nr_mul2(a, c[e]));
+                            f[2 + e] = nr_fma2(a, s[e], nr_mul2(b, c[e]));
+                        }
                     }
                 } else if constexpr (MODE == ROPE_ANY) {
                     // the partner of a channel may sit in any lane: through shared memory
@@ -217,9 +230,10 @@ __global__ void __launch_bounds__(NR_THREADS, 8) norm_rope_kernel(const NormRope
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         auto partner = [&](int d) {
-                            return d >= p.rot ? d : !p.neox ? d ^ 1 : d < half ? d + half : d - half;
+                            return !p.neox ? d ^ 1 : d < half ? d + half : d - half;
                         };
                         const int d = 8 * lane + 2 * e;
+                        if (d >= p.rot) break;              // (rot is even)
                         f[e] = nr_fma2(make_float2(row[partner(d)], row[partner(d + 1)]), s[e],
                                        nr_mul2(f[e], c[e]));
                     }
@@ -230,10 +244,10 @@ __global__ void __launch_bounds__(NR_THREADS, 8) norm_rope_kernel(const NormRope
                                    pack_bf16x2(f[2].x, f[2].y), pack_bf16x2(f[3].x, f[3].y));
             }
             if (is_q && h < end) {
-                *reinterpret_cast<uint4*>(p.q_out + t * p.o_tok + h * p.o_head + 8 * lane) = y;
+                store_row(p.q_out + t * p.o_tok + h * p.o_head, y);
             } else if (h < end && stored) {
-                *reinterpret_cast<uint4*>(is_k ? p.k_cache + at + (h - p.H) * p.ch
-                                               : p.v_cache + at + (h - qk) * p.ch) = y;
+                store_row(is_k ? p.k_cache + at + (h - p.H) * p.ch
+                               : p.v_cache + at + (h - qk) * p.ch, y);
             }
         }
     }
@@ -315,16 +329,14 @@ extern "C" int locks_norm_rope_write(
     p.n_tok = n_tok; p.H = n_heads; p.n_kv = n_kv; p.eps = eps;
     int mode = ROPE_NONE;
     if (cos_sin) {
-        // vector loads of a lane's table values: 8 (half-split) or 4 (interleaved)
-        // in a row, starting at a multiple of that many and `half` behind it
+        // vector loads of a lane's table values: four in a row, starting at a multiple
+        // of four and `half` behind it
         const int align = table_f32 ? 16 : 8;
         const int es = table_f32 ? 4 : 2, half = rot_dim / 2;
         const bool vec = reinterpret_cast<uintptr_t>(cos_sin) % align == 0 &&
                          (cos_sin_row_stride * es) % align == 0 &&
                          (half * es) % align == 0;
-        mode = !vec ? ROPE_ANY
-               : neox ? (half % 8 == 0 ? ROPE_HALVES : ROPE_ANY)
-                      : (rot_dim % 8 == 0 ? ROPE_PAIRS : ROPE_ANY);
+        mode = !vec || rot_dim % 8 != 0 ? ROPE_ANY : neox ? ROPE_HALVES : ROPE_PAIRS;
     }
     // A token to a warp when that fills the device about once (32 warps to an SM); else
     // its heads are shared by more warps, down to one step each.  16384 tokens x 36 heads:
