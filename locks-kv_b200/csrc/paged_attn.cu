@@ -69,7 +69,7 @@ extern "C" int locks_window_attention(
     p.v = static_cast<const __nv_bfloat16*>(v_cache);
     p.sb = kv_stride_block; p.st = kv_stride_tok; p.sh = kv_stride_head;
     p.table = block_table; p.bt_stride = bt_stride; p.bt_width = bt_width;
-    p.num_blocks = num_blocks; p.cu_q = cu_q; p.seq_lens = seq_lens;
+    p.num_blocks = num_blocks; p.n_tok = n_tok; p.cu_q = cu_q; p.seq_lens = seq_lens;
     p.out = static_cast<__nv_bfloat16*>(out); p.o_tok = o_stride_tok; p.o_head = o_stride_head;
     p.lse = lse; p.lse_tok = lse_stride_tok;
     p.n_kv = n_kv; p.G = G; p.window = window; p.sinks = sinks;
@@ -131,7 +131,7 @@ extern "C" int locks_shared_prefix_decode(
     p.v = static_cast<const __nv_bfloat16*>(v_cache);
     p.sb = kv_stride_block; p.st = kv_stride_tok; p.sh = kv_stride_head;
     p.table = block_table; p.bt_stride = bt_stride; p.bt_width = bt_width;
-    p.num_blocks = num_blocks; p.seq_lens = seq_lens;
+    p.num_blocks = num_blocks; p.n_tok = n_req; p.seq_lens = seq_lens;
     p.out = static_cast<__nv_bfloat16*>(out); p.o_tok = o_stride_req; p.o_head = o_stride_head;
     p.lse = lse; p.lse_tok = lse_stride_req;
     p.n_kv = n_kv; p.G = G; p.window = INT32_MAX; p.sinks = 0;

@@ -112,7 +112,7 @@ struct RowAttnParams {
     int64_t sb, st, sh;               // cache strides: block, token, KV head
     const int32_t* table;
     int64_t bt_stride;
-    int bt_width, num_blocks;
+    int bt_width, num_blocks, n_tok;  // n_tok: rows of q and out
     const int32_t* cu_q;              // null: request r's one token is row r
     const int32_t* seq_lens;
     __nv_bfloat16* out;
@@ -145,7 +145,6 @@ struct TileAttnParams {
     float *parts_out, *parts_ml;
     int* status;
     int head_chunks;                  // 64-channel chunks between two heads
-    int max_tiles;                    // upper bound of the row tiles of all segments
 };
 
 // csrc/row_attn.cu; `who` names the entry point in error messages, no request has more

@@ -110,7 +110,8 @@ __global__ void __launch_bounds__(WARPS * 32) row_attn_kernel(const RowAttnParam
     }
     const int tok0 = p.cu_q ? p.cu_q[r] : r;
     const int n_q = p.cu_q ? p.cu_q[r + 1] - tok0 : 1;
-    const int rows = n_q * G;
+    // (bounds that leave q are cut off; n_q still says where the request's queries sit)
+    const int rows = tok0 < 0 ? 0 : min(n_q, p.n_tok - tok0) * G;
     if (rows > p.max_rows) {                  // the tiled kernel's
         pdl_wait();
         return;

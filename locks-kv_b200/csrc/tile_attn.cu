@@ -174,23 +174,45 @@ __device__ __forceinline__ void tma_load_rows(void* dst, const CUtensorMap* map,
 // segment s: first token and token count (0 where the few-row kernel serves it)
 __device__ __forceinline__ void segment(const TileAttnParams& p, int s, int& t0, int& n) {
     t0 = p.bounds[s];
-    n = p.bounds[s + 1] - t0;
-    if (!p.prefix_lens && n * p.r.G <= p.min_rows) n = 0;
+    n = min(p.bounds[s + 1], p.r.n_tok) - t0;
+    if (t0 < 0 || (!p.prefix_lens && n * p.r.G <= p.min_rows)) n = 0;
     n = max(n, 0);
 }
+__device__ __forceinline__ int tiles_of(const TileAttnParams& p, int n) {
+    return (n * p.r.G + 2 * TA_TILE - 1) / (2 * TA_TILE);
+}
 
-// Work item `w` (tile of a segment fastest, then KV head, then part), by one warp;
-// false: there is no such tile.
-__device__ __forceinline__ bool find_item(const TileAttnParams& p, int w, int lane, Item& it) {
-    const int target = w % p.max_tiles, rest = w / p.max_tiles;
-    int before = 0;
-    for (int s0 = 0; s0 < p.n_seg; s0 += 32) {
-        int t0 = 0, n = 0, extent = 0;
+// tiles of all segments, by one warp
+__device__ __forceinline__ int count_tiles(const TileAttnParams& p, int lane) {
+    int sum = 0;
+#pragma unroll 4
+    for (int s = lane; s < p.n_seg; s += 32) {
+        int t0, n;
+        segment(p, s, t0, n);
+        sum += tiles_of(p, n);
+    }
+    return __reduce_add_sync(0xffffffffu, sum);
+}
+
+// Where a search for tiles stands: segments from s0 on begin with tile number `before`.
+struct FindState {
+    int s0, before;
+};
+
+// Work item `w` of `total` tiles x KV heads x parts, tiles fastest, by one warp.
+__device__ __forceinline__ void find_item(const TileAttnParams& p, int w, int total, int lane,
+                                          FindState& at, Item& it) {
+    const int target = w % total, rest = w / total;
+    if (target < at.before) at = {0, 0};
+    for (; at.s0 < p.n_seg; at.s0 += 32) {
+        const int s0 = at.s0, before = at.before;
+        int t0 = 0, n = 0, extent = 0, end = 0;
         if (s0 + lane < p.n_seg) {
             extent = p.prefix_lens ? p.prefix_lens[s0 + lane] : p.r.seq_lens[s0 + lane];
             segment(p, s0 + lane, t0, n);
+            end = p.bounds[s0 + lane + 1];
         }
-        const int mine = (n * p.r.G + 2 * TA_TILE - 1) / (2 * TA_TILE);
+        const int mine = tiles_of(p, n);
         int x = mine;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
@@ -220,7 +242,8 @@ __device__ __forceinline__ bool find_item(const TileAttnParams& p, int w, int la
                 it.list = page_list(0, it.key_end - 1, INT32_MAX, 0, p.r.bt_width);
             } else {
                 it.written = extent;
-                it.base_pos = it.written - n;
+                // (where the queries sit goes by the bounds, cut off or not)
+                it.base_pos = it.written - (__shfl_sync(0xffffffffu, end, src) - it.t0);
                 it.table_row = it.seg;
                 it.list = page_list(it.base_pos + it.row0 / G,
                                     it.base_pos + (it.row0 + it.n_rows - 1) / G, p.r.window,
@@ -232,11 +255,10 @@ __device__ __forceinline__ bool find_item(const TileAttnParams& p, int w, int la
             it.j0 = min(it.part * per, all);
             it.n_tiles = min(it.j0 + per, all) - it.j0;
             it.valid = 1;
-            return true;
+            return;
         }
-        before += __shfl_sync(0xffffffffu, x, 31);
+        at.before += __shfl_sync(0xffffffffu, x, 31);
     }
-    return false;
 }
 
 __global__ void __launch_bounds__(TA_THREADS, 1)
@@ -294,12 +316,13 @@ tile_attn_kernel(const __grid_constant__ CUtensorMap map_q,
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
         if (warp == 10) {
             // ---- items ----------------------------------------------------------------
-            const int total = p.max_tiles * p.r.n_kv * p.parts;
+            const int tiles = count_tiles(p, lane), total = tiles * p.r.n_kv * p.parts;
+            FindState at = {0, 0};
             int n = 0;
             for (int w = blockIdx.x; !__any_sync(0xffffffffu, is_dead(sm)); w += gridDim.x) {
                 Item it;
                 it.valid = 0;
-                if (w < total && !find_item(p, w, lane, it)) continue;
+                if (w < total) find_item(p, w, tiles, lane, at, it);
                 if (n >= 2)
                     ta_wait(sm, &sm.item_empty[n & 1], (uint32_t)((n >> 1) - 1) & 1u, p.status);
                 if (lane == 0) {
@@ -869,7 +892,9 @@ __global__ void __launch_bounds__(32 * TJ_WARPS) join_parts_kernel(const TileAtt
             const int mid = (lo + hi) >> 1;
             if (p.bounds[mid + 1] > tok) hi = mid; else lo = mid + 1;
         }
-        if ((p.bounds[lo + 1] - p.bounds[lo]) * p.r.G <= p.min_rows) return;
+        int t0, n;
+        segment(p, lo, t0, n);
+        if (n == 0) return;                         // the few-row kernel's
     }
     const PartSum s = join_parts(p.parts_out, p.parts_ml, p.part_rows, parts, at, 4 * lane);
     const float inv = s.l > 0.f ? 1.f / s.l : 0.f;
@@ -886,7 +911,6 @@ __global__ void __launch_bounds__(32 * TJ_WARPS) join_parts_kernel(const TileAtt
 int launch_tile_attn(const char* who, TileAttnParams p, int max_tiles, int n_tok,
                      cudaStream_t s) {
     p.head_chunks = p.r.n_kv > 1 ? (int)(p.r.sh / 64) : 0;
-    p.max_tiles = max_tiles;
     CUtensorMap mq = {}, mk, mv;
     CUresult cr = TA_TILE % p.r.G == 0 ? encode_q(&mq, p.r, n_tok) : CUDA_SUCCESS;
     if (cr == CUDA_SUCCESS)

@@ -121,6 +121,8 @@ def norm_rope_and_cache(q: torch.Tensor, key: torch.Tensor, val: torch.Tensor,
     assert qs[2] == ks[2] == vs[2] == os[2] == cs[3] == 1
     assert slot_mapping.dtype is i64 and slot_mapping.is_contiguous()
     assert slot_mapping.numel() >= n_tok
+    if n_tok == 0:
+        return q_out
     rot = rows = row_stride = t_f32 = 0
     if cos_sin is not None:
         assert positions is not None and positions.dtype is i64

@@ -1,6 +1,10 @@
 """Attention over the paged cache outside the page selection: sliding window with
 first tokens kept visible, and decode of a batch that shares long prefixes (host
-wrappers of ``locks_window_attention`` and ``locks_shared_prefix_decode``)."""
+wrappers of ``locks_window_attention`` and ``locks_shared_prefix_decode``).
+
+Caches come in either engine layout, (NB, 2, page, n_kv, d) or (2, NB, page, n_kv, d),
+with any strides whose rows are 16-byte aligned and whose head stride is a multiple
+of 64 (a head-major view too); one of exactly two blocks is read as the latter."""
 from __future__ import annotations
 
 from typing import Optional
@@ -65,6 +69,8 @@ def window_paged_attention(q: torch.Tensor, kv_cache: torch.Tensor,
                                        n_kv, G, (cu_q, seq_lens))
     R = seq_lens.numel()
     assert cu_q.numel() == R + 1 and block_table.shape[0] == R
+    if R == 0 or q.shape[0] == 0:
+        return
     _cabi.call_on(dev, "locks_window_attention", *source, cu_q.data_ptr(),
                   seq_lens.data_ptr(), *target, q.shape[0], R, max_q, n_kv, G, d, page,
                   NO_WINDOW if window is None else min(window, NO_WINDOW), sinks,
@@ -91,6 +97,8 @@ def shared_prefix_paged_decode(q: torch.Tensor, kv_cache: torch.Tensor,
     R, groups = q.shape[0], prefix_lens.numel()
     assert seq_lens.numel() == block_table.shape[0] == R
     assert cu_groups.numel() == groups + 1
+    if R == 0 or groups == 0:
+        return
     _cabi.call_on(dev, "locks_shared_prefix_decode", *source, seq_lens.data_ptr(),
                   cu_groups.data_ptr(), prefix_lens.data_ptr(), *target, R, groups,
                   n_kv, G, d, page, scale, _cabi.addr(status))

@@ -25,7 +25,7 @@ def i32(x):
 def run_plan(lens, new, table, free, taken, cap, *, page=16, in_place=False):
     from locks.attention import append_plan
     R = len(lens)
-    t = dict(lens=i32(lens), new=i32(new), table=i32(table).reshape(R, -1), free=i32(free),
+    t = dict(lens=i32(lens), new=i32(new), table=i32(table).reshape(R, len(table[0])), free=i32(free),
              taken=i32([taken]), status=i32([0]))
     o = dict(slots=torch.full((cap,), 77, dtype=I64, device=DEV),
              pos=torch.full((cap,), 77, dtype=I64, device=DEV),
@@ -270,6 +270,101 @@ def test_window_short_table_and_small_bound():
         at = slice(cu[r], cu[r + 1])
         check(out[at], None, want_window(q[at], k, v, table[r], lens[r], cu[r + 1] - cu[r],
                                          2 ** 31 - 1, 0))
+
+
+def test_window_many_requests_few_of_them_long():
+    """Several hundred requests, most with one token, prompts between them."""
+    n_kv, G, R = 1, 8, 700
+    rng = random.Random(5)
+    n_q = [1] * R
+    for r in (3, 31, 32, 500, 699):
+        n_q[r] = rng.choice([17, 64, 129])
+    lens = [n + rng.randrange(60) for n in n_q]
+    g, cache, k, v, table = paged(11, lens, n_kv)
+    cu = [0]
+    for n in n_q:
+        cu.append(cu[-1] + n)
+    q = torch.randn(cu[-1], G, 128, device=DEV, generator=g).to(BF16)
+    out = run_window(q, cache, table, i32(cu), i32(lens), n_kv, G, 40, 3, max(n_q))
+    for r in (0, 3, 4, 31, 32, 33, 499, 500, 501, 698, 699):
+        at = slice(cu[r], cu[r + 1])
+        check(out[at], None, want_window(q[at], k, v, table[r], lens[r], n_q[r], 40, 3), r)
+    assert bool(out.isfinite().all())
+
+
+def test_window_head_major_cache_strided_table_and_no_programmatic_launch():
+    """Heads outside tokens in storage, a table that is a view, G that does not divide
+    128, and the launches without their programmatic edge: the same numbers."""
+    from locks import _cabi
+    n_kv, G, reqs = 3, 6, [(1, 500), (90, 300), (2, 33)]
+    g, cache, k, v, table = paged(12, [l for _, l in reqs], n_kv)
+    other = cache.transpose(2, 3).contiguous().transpose(2, 3)
+    wide = torch.full((3, table.shape[1] + 5), -7, dtype=I32, device=DEV)
+    wide[:, 2:-3] = table
+    q = torch.randn(93, 18, 128, device=DEV, generator=g).to(BF16)
+    cu, lens = i32([0, 1, 91, 93]), i32([l for _, l in reqs])
+    a = run_window(q, cache, table, cu, lens, n_kv, G, 100, 9, 90)
+    old = _cabi.lib().locks_set_pdl(0)
+    try:
+        b = run_window(q, other, wide[:, 2:-3], cu, lens, n_kv, G, 100, 9, 90)
+        torch.cuda.synchronize()
+    finally:
+        _cabi.lib().locks_set_pdl(old)
+    assert torch.equal(a, b)
+    check(a[1:91], None, want_window(q[1:91], k, v, table[1], 300, 90, 100, 9))
+
+
+def test_offsets_beyond_31_bits():
+    """Blocks whose element offsets pass 2^31: attention of both kinds, and the write."""
+    from locks.attention import norm_rope_and_cache
+    n_kv, G, NB = 8, 2, 66000
+    cache = torch.zeros(NB, 2, 16, n_kv, 128, device=DEV, dtype=BF16)
+    g = torch.Generator(device=DEV).manual_seed(3)
+    far = torch.arange(NB - 20, NB, device=DEV)
+    cache[far] = torch.randn(20, 2, 16, n_kv, 128, device=DEV, generator=g).to(BF16)
+    table = far.to(I32).reshape(2, 10)
+    q = torch.randn(40, 16, 128, device=DEV, generator=g).to(BF16)
+    cu, lens = [0, 1, 40], [160, 150]
+    out = run_window(q, cache, table, i32(cu), i32(lens), n_kv, G, 70, 5, 39)
+    for r in range(2):
+        at = slice(cu[r], cu[r + 1])
+        check(out[at], None, want_window(q[at], cache[:, 0], cache[:, 1], table[r], lens[r],
+                                         cu[r + 1] - cu[r], 70, 5))
+    two = run_prefix(q[:2], cache, table[:1].expand(2, -1), [160, 133], [0, 2], [128], n_kv, G)
+    for r, l in enumerate((160, 133)):
+        check(two[r:r + 1], None, want_window(q[r:r + 1], cache[:, 0], cache[:, 1], table[0], l, 1,
+                                              2 ** 31 - 1, 0))
+    kv = torch.randn(1, 2 * n_kv, 128, device=DEV, generator=g).to(BF16)
+    slot = torch.tensor([NB * 16 - 1], device=DEV)
+    norm_rope_and_cache(q[:1], kv[:, :n_kv], kv[:, n_kv:], cache, slot, None, None)
+    assert torch.equal(cache[-1, 0, 15], kv[0, :n_kv]) and torch.equal(cache[-1, 1, 15], kv[0, n_kv:])
+
+
+def test_empty_batches():
+    from locks.attention import norm_rope_and_cache
+    g, cache, k, v, table = paged(2, [20], 2)
+    none, q = i32([]), torch.zeros(0, 8, 128, device=DEV, dtype=BF16)
+    run_window(q, cache, table[:0], i32([0]), none, 2, 4, 10, 0, 0)
+    run_window(q, cache, table, i32([0, 0]), i32([20]), 2, 4, 10, 0, 0)
+    run_prefix(q, cache, table[:0], [], [0], [], 2, 4, floats=16)
+    norm_rope_and_cache(q, q[:, :2], q[:, :2], cache, torch.zeros(0, dtype=I64, device=DEV), None, None)
+    got = run_plan([], [], [[]], [4], 1, 3)
+    assert got["slots"] == [-1] * 3 and got["taken"] == 1 and got["cu"] == [0]
+
+
+def test_bounds_beyond_the_queries_are_cut_off():
+    """cu_q that runs past q (fewer rows than it says): the rows that exist are right,
+    nothing behind them is touched."""
+    n_kv, G = 2, 4
+    g, cache, k, v, table = paged(21, [90, 50], n_kv)
+    q = torch.randn(64, 8, 128, device=DEV, generator=g).to(BF16)
+    out = torch.full((64, 8, 128), 7.0, device=DEV, dtype=BF16)
+    run_window(q[:50], cache, table, i32([0, 40, 80]), i32([90, 50]), n_kv, G, None, 0, 40,
+               out=out[:50])
+    assert bool((out[50:] == 7).all())
+    check(out[:40], None, want_window(q[:40], k, v, table[0], 90, 40, 2 ** 31 - 1, 0))
+    want = want_window(q[40:64], k, v, table[1], 50 - 16, 24, 2 ** 31 - 1, 0)
+    check(out[40:50], None, [x[:10] for x in want])
 
 
 def test_window_repeats_bit_for_bit_on_another_stream():

@@ -74,7 +74,8 @@ SHARED = [(dict(q=None), -1, "null"), (dict(lens=None), -1, "null"), (dict(cu=No
           (dict(d=64), -2, "head_dim"), (dict(page=8), -2, "page"), (dict(G=17), -2, "G <= 16"),
           (dict(G=0), -2, "G <= 16"), (dict(st=252), -1, "aligned"), (dict(q=ODD), -1, "aligned"),
           (dict(out=ODD), -1, "aligned"), (dict(scratch=ODD), -1, "aligned"), (dict(n_kv=0), -1, "size"),
-          (dict(sh=136), -2, "multiple of 64"), (dict(sb=0), -1, "stride"), (dict(width=0), -1, "size"), (dict(n_req=65536), -1, "size"), (dict(n_req=0), 0, "")]
+          (dict(sh=136), -2, "multiple of 64"), (dict(sb=0), -1, "stride"), (dict(scale=0.0), -1, "positive"),
+          (dict(scale=float("nan")), -1, "positive"), (dict(width=0), -1, "size"), (dict(n_req=65536), -1, "size"), (dict(n_req=0), 0, "")]
 
 
 @pytest.mark.parametrize("change,code,word", SHARED + [
