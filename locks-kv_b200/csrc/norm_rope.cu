@@ -12,9 +12,12 @@
 // in a row (one 16-byte access), or in half-split pairing four of each half (two of 8
 // bytes), so that both channels of a pair are its own.  A warp takes one token
 // (or, where there are few tokens, a share of its heads), whose slot, position and
-// (cos | sin) row it reads once, in steps of NR_ROWS pairs of neighbouring rows; the
-// next step's rows are on their way while a step is computed.  Pairs of channels share
+// (cos | sin) row it reads once, and goes through its query, key and value heads in steps
+// of NR_ROWS pairs of neighbouring rows; the next step's rows are on their way while a
+// step is computed.  Pairs of channels share
 // an instruction (fp32x2), which keeps the arithmetic below the memory time.
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace locks {
@@ -93,7 +96,7 @@ __global__ void __launch_bounds__(NR_THREADS, 8) norm_rope_kernel(const NormRope
     const int job = blockIdx.x * (NR_THREADS / 32) + (threadIdx.x >> 5);
     const int t = job / p.shares;
     if (t >= p.n_tok) return;                    // (a whole warp)
-    int h0 = (job - t * p.shares) * p.share;     // the warp's heads [h0, end)
+    const int h0 = (job - t * p.shares) * p.share;     // the warp's heads [h0, end)
     const int end = min(h0 + p.share, heads);
     // the lane's channels: [ca, ca + 4) and [cb, cb + 4).  Half-split: of either half
     // while there are rotated ones, the rest in order
@@ -118,25 +121,6 @@ __global__ void __launch_bounds__(NR_THREADS, 8) norm_rope_kernel(const NormRope
             *reinterpret_cast<uint4*>(row + ca) = y;
         }
     };
-    const __nv_bfloat16* q = p.q + t * p.q_tok;
-    const __nv_bfloat16* k = p.k + t * p.k_tok;
-    const __nv_bfloat16* v = p.v + t * p.v_tok;
-
-    uint4 next[NR_ROWS];
-    auto fetch = [&](int first) {
-#pragma unroll
-        for (int i = 0; i < NR_ROWS; ++i) {
-            const int h = first + 2 * i + side;
-            if (h >= end) continue;
-            const __nv_bfloat16* src = h < p.H ? q + h * p.q_head
-                                       : h < qk ? k + (h - p.H) * p.k_head
-                                                : v + (h - qk) * p.v_head;
-            next[i] = load_row(src);
-        }
-    };
-#pragma unroll
-    for (int i = 0; i < NR_ROWS; ++i) next[i] = make_uint4(0, 0, 0, 0);
-    fetch(h0);
     const int64_t slot = p.slot[t];
     // the token's table row, as far as this lane's channels need it
     const Tab* cs = static_cast<const Tab*>(p.cos_sin);
@@ -166,91 +150,118 @@ __global__ void __launch_bounds__(NR_THREADS, 8) norm_rope_kernel(const NormRope
     }
     const bool stored = slot >= 0 && (slot >> 4) < p.num_blocks;
     const int64_t at = stored ? (slot >> 4) * p.cb + (slot & 15) * p.ct : 0;
-    for (; h0 < end; h0 += 2 * NR_ROWS) {
-        uint4 x[NR_ROWS];
-#pragma unroll
-        for (int i = 0; i < NR_ROWS; ++i) x[i] = next[i];
-        if (h0 + 2 * NR_ROWS < end) fetch(h0 + 2 * NR_ROWS);
-#pragma unroll
-        for (int i = 0; i < NR_ROWS; ++i) {
-            const int h = h0 + 2 * i + side;
-            const bool is_q = h < p.H, is_k = !is_q && h < qk;
-            uint4 y = x[i];
-            // (both half-warps of a warp come along: the shuffles need all lanes)
-            if (h0 + 2 * i < qk) {
-                const uint32_t raw[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-                float2 f[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) f[e] = unpack2(raw[e]);
-                const void* wt = is_q ? p.q_weight : is_k ? p.k_weight : nullptr;
-                float2 sq = nr_mul2(f[0], f[0]);
-#pragma unroll
-                for (int e = 1; e < 4; ++e) sq = nr_fma2(f[e], f[e], sq);
-                float ss = sq.x + sq.y;
-#pragma unroll
-                for (int d = 1; d < 16; d <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
-                if (wt) {
-                    const float rs = rsqrtf(ss * (1.f / NR_HD) + p.eps);
-                    float2 w[2];
-#pragma unroll
-                    for (int e = 0; e < 4; e += 2) {
-                        const int ch = e ? cb : ca;
-                        if (p.weight_f32) load_vals(static_cast<const float*>(wt) + ch, w);
-                        else load_vals(static_cast<const __nv_bfloat16*>(wt) + ch, w);
-                        f[e] = nr_mul2(nr_mul2(f[e], make_float2(rs, rs)), w[0]);
-                        f[e + 1] = nr_mul2(nr_mul2(f[e + 1], make_float2(rs, rs)), w[1]);
-                    }
-                }
-                if constexpr (MODE == ROPE_PAIRS) {
-                    if (turns) {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float ce = e & 1 ? c[e >> 1].y : c[e >> 1].x;
-                            const float se = e & 1 ? s[e >> 1].y : s[e >> 1].x;
-                            f[e] = nr_fma2(make_float2(f[e].y, f[e].x), make_float2(-se, se),
-                                           nr_mul2(f[e], make_float2(ce, ce)));
-                        }
-                    }
-                } else if constexpr (MODE == ROPE_HALVES) {
-                    if (turns) {
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            const float2 a = f[e], b = f[2 + e];
-                            f[e] = nr_fma2(b, make_float2(-s[e].x, -s[e].y), nr_mul2(a, c[e]));
-                            f[2 + e] = nr_fma2(a, s[e], nr_mul2(b, c[e]));
-                        }
-                    }
-                } else if constexpr (MODE == ROPE_ANY) {
-                    // the partner of a channel may sit in any lane: through shared memory
-                    float* row = stage[half_id];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        *reinterpret_cast<float2*>(&row[8 * lane + 2 * e]) = f[e];
-                    __syncwarp();
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        auto partner = [&](int d) {
-                            return !p.neox ? d ^ 1 : d < half ? d + half : d - half;
-                        };
-                        const int d = 8 * lane + 2 * e;
-                        if (d >= p.rot) break;              // (rot is even)
-                        f[e] = nr_fma2(make_float2(row[partner(d)], row[partner(d + 1)]), s[e],
-                                       nr_mul2(f[e], c[e]));
-                    }
-                    __syncwarp();
-                }
-                if (h < qk)
-                    y = make_uint4(pack_bf16x2(f[0].x, f[0].y), pack_bf16x2(f[1].x, f[1].y),
-                                   pack_bf16x2(f[2].x, f[2].y), pack_bf16x2(f[3].x, f[3].y));
-            }
-            if (is_q && h < end) {
-                store_row(p.q_out + t * p.o_tok + h * p.o_head, y);
-            } else if (h < end && stored) {
-                store_row(is_k ? p.k_cache + at + (h - p.H) * p.ch
-                               : p.v_cache + at + (h - qk) * p.ch, y);
+    // Heads [from, to) of one kind: rows `src_step` / `dst_step` apart, the half-warp's own
+    // every second one.  turn: norm (with a weight) and rotation, else a copy.
+    auto heads_of = [&](auto turn, int from, int to, const __nv_bfloat16* src, int64_t src_step,
+                        __nv_bfloat16* dst, int64_t dst_step, const void* weight, bool store) {
+        if (from >= to) return;
+        const int mine = (to - from - side + 1) >> 1, pairs = (to - from + 1) >> 1;
+        src += side * src_step;
+        dst += side * dst_step;
+        src_step *= 2;
+        dst_step *= 2;
+        float2 w[4];
+        if (decltype(turn)::value && weight) {
+            float2 (&wa)[2] = reinterpret_cast<float2 (&)[2]>(w[0]);
+            float2 (&wb)[2] = reinterpret_cast<float2 (&)[2]>(w[2]);
+            if (p.weight_f32) {
+                load_vals(static_cast<const float*>(weight) + ca, wa);
+                load_vals(static_cast<const float*>(weight) + cb, wb);
+            } else {
+                load_vals(static_cast<const __nv_bfloat16*>(weight) + ca, wa);
+                load_vals(static_cast<const __nv_bfloat16*>(weight) + cb, wb);
             }
         }
-    }
+        uint4 next[NR_ROWS];
+#pragma unroll
+        for (int i = 0; i < NR_ROWS; ++i) {
+            next[i] = make_uint4(0, 0, 0, 0);
+            if (i < mine) next[i] = load_row(src + i * src_step);
+        }
+        for (int j = 0; j < pairs; j += NR_ROWS) {
+            uint4 x[NR_ROWS];
+#pragma unroll
+            for (int i = 0; i < NR_ROWS; ++i) x[i] = next[i];
+            src += NR_ROWS * src_step;
+#pragma unroll
+            for (int i = 0; i < NR_ROWS; ++i)
+                if (j + NR_ROWS + i < mine) next[i] = load_row(src + i * src_step);
+#pragma unroll
+            for (int i = 0; i < NR_ROWS; ++i) {
+                // (both half-warps come along: the shuffles need all lanes)
+                uint4 y = x[i];
+                if constexpr (decltype(turn)::value) {
+                    const uint32_t raw[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+                    float2 f[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) f[e] = unpack2(raw[e]);
+                    if (weight) {
+                        float2 sq = nr_mul2(f[0], f[0]);
+#pragma unroll
+                        for (int e = 1; e < 4; ++e) sq = nr_fma2(f[e], f[e], sq);
+                        float ss = sq.x + sq.y;
+#pragma unroll
+                        for (int d = 1; d < 16; d <<= 1)
+                            ss += __shfl_xor_sync(0xffffffffu, ss, d);
+                        const float rs = rsqrtf(ss * (1.f / NR_HD) + p.eps);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            f[e] = nr_mul2(nr_mul2(f[e], make_float2(rs, rs)), w[e]);
+                    }
+                    if constexpr (MODE == ROPE_PAIRS) {
+                        if (turns) {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const float ce = e & 1 ? c[e >> 1].y : c[e >> 1].x;
+                                const float se = e & 1 ? s[e >> 1].y : s[e >> 1].x;
+                                f[e] = nr_fma2(make_float2(f[e].y, f[e].x), make_float2(-se, se),
+                                               nr_mul2(f[e], make_float2(ce, ce)));
+                            }
+                        }
+                    } else if constexpr (MODE == ROPE_HALVES) {
+                        if (turns) {
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                const float2 a = f[e], b = f[2 + e];
+                                f[e] = nr_fma2(b, make_float2(-s[e].x, -s[e].y), nr_mul2(a, c[e]));
+                                f[2 + e] = nr_fma2(a, s[e], nr_mul2(b, c[e]));
+                            }
+                        }
+                    } else if constexpr (MODE == ROPE_ANY) {
+                        // the partner of a channel may sit in any lane: through shared memory
+                        float* row = stage[half_id];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            *reinterpret_cast<float2*>(&row[8 * lane + 2 * e]) = f[e];
+                        __syncwarp();
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            auto partner = [&](int d) {
+                                return !p.neox ? d ^ 1 : d < half ? d + half : d - half;
+                            };
+                            const int d = 8 * lane + 2 * e;
+                            if (d >= p.rot) break;          // (rot is even)
+                            f[e] = nr_fma2(make_float2(row[partner(d)], row[partner(d + 1)]),
+                                           s[e], nr_mul2(f[e], c[e]));
+                        }
+                        __syncwarp();
+                    }
+                    y = make_uint4(pack_bf16x2(f[0].x, f[0].y), pack_bf16x2(f[1].x, f[1].y),
+                                   pack_bf16x2(f[2].x, f[2].y), pack_bf16x2(f[3].x, f[3].y));
+                }
+                if (store && j + i < mine) store_row(dst + i * dst_step, y);
+            }
+            dst += NR_ROWS * dst_step;
+        }
+    };
+    const int64_t tq = t * p.q_tok, to = t * p.o_tok, tk = t * p.k_tok, tv = t * p.v_tok;
+    const int k0 = max(h0, p.H), v0 = max(h0, qk);
+    heads_of(std::true_type{}, h0, min(end, p.H), p.q + tq + h0 * p.q_head, p.q_head,
+             p.q_out + to + h0 * p.o_head, p.o_head, p.q_weight, true);
+    heads_of(std::true_type{}, k0, min(end, qk), p.k + tk + (k0 - p.H) * p.k_head, p.k_head,
+             p.k_cache + at + (k0 - p.H) * p.ch, p.ch, p.k_weight, stored);
+    heads_of(std::false_type{}, v0, end, p.v + tv + (v0 - qk) * p.v_head, p.v_head,
+             p.v_cache + at + (v0 - qk) * p.ch, p.ch, nullptr, stored);
 }
 
 template <class Tab>
