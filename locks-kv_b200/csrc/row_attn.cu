@@ -386,15 +386,31 @@ __global__ void __launch_bounds__(WARPS * 32) row_attn_kernel(const RowAttnParam
 }
 
 template <int WARPS, int STAGES, bool CLUSTER, bool HI>
-int launch_row(const char* who, const RowAttnParams& p, int n_req, int cl, cudaStream_t s) {
+int launch_row(const char* who, const RowAttnParams& p, int n_req, cudaStream_t s) {
     auto kernel = row_attn_kernel<WARPS, STAGES, CLUSTER, HI>;
+    // clusters of 2, 4, 8 and 16 CTAs the device holds at once (a cluster lives in one
+    // GPC, so that fewer of the large ones fit than SMs would suggest)
+    static int fit[64][4] = {};
     static bool attr_done[64] = {false};
     int dev = 0;
     cudaGetDevice(&dev);
     const int smem = (int)sizeof(RowSmem<WARPS, STAGES, CLUSTER>);
-    if (dev >= 0 && dev < 64 && !attr_done[dev]) {
+    const bool known = dev >= 0 && dev < 64;
+    if (known && !attr_done[dev]) {
         cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (CLUSTER) {
+            cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+            for (int i = 0; i < 4; ++i)
+                fit[dev][i] = max_active_clusters(kernel, 2 << i, WARPS * 32, smem);
+        }
         attr_done[dev] = true;
+    }
+    int cl = 1;
+    if (CLUSTER) {
+        // the largest that lets every pair's cluster run at once
+        cl = 2;
+        for (int i = 1; i < 4; ++i)
+            if (known && (int64_t)n_req * p.n_kv <= fit[dev][i]) cl = 2 << i;
     }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(cl, p.n_kv, n_req);
@@ -435,12 +451,10 @@ int launch_row_attn(const char* who, const RowAttnParams& p, int n_req, int most
     const int64_t pairs = (int64_t)n_req * p.n_kv;
     const bool hi = most_rows > 8;
     if (2 * pairs > sm_count())
-        return hi ? launch_row<4, 3, false, true>(who, p, n_req, 1, s)
-                  : launch_row<4, 3, false, false>(who, p, n_req, 1, s);
-    int cl = 2;
-    while (cl < 8 && cl * 2 * pairs <= sm_count()) cl *= 2;
-    return hi ? launch_row<8, 2, true, true>(who, p, n_req, cl, s)
-              : launch_row<8, 2, true, false>(who, p, n_req, cl, s);
+        return hi ? launch_row<4, 3, false, true>(who, p, n_req, s)
+                  : launch_row<4, 3, false, false>(who, p, n_req, s);
+    return hi ? launch_row<8, 2, true, true>(who, p, n_req, s)
+              : launch_row<8, 2, true, false>(who, p, n_req, s);
 }
 
 }  // namespace locks
