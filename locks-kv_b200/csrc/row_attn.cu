@@ -24,8 +24,8 @@
 //                                   of the output each -- no partials in HBM, one launch.
 //
 // P is split into two bf16 terms (P = hi + lo to 2^-17), so the product with V
-// loses nothing to P's rounding; the second product costs tensor time that the
-// memory-bound loop has to spare.  Keys that no row sees are filled with zeros
+// loses nothing to P's rounding; with up to 8 rows both terms share one product, above
+// the second one costs tensor time that the memory-bound loop has to spare.  Keys that no row sees are filled with zeros
 // on the way in, so what the cache holds there cannot reach the result.
 //
 // Behind the tiled kernel of the same call it is launched programmatically: it starts on
@@ -207,7 +207,9 @@ __global__ void __launch_bounds__(WARPS * 32) row_attn_kernel(const RowAttnParam
             __syncwarp();
             const uint32_t kbase = smem_u32(&sm.wb[warp].k[stage]);
             const uint32_t vbase = smem_u32(&sm.wb[warp].v[stage]);
+            // (two chains of products per half page: each is latency, not work)
             float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
+            float u0[4] = {0.f, 0.f, 0.f, 0.f}, u1[4] = {0.f, 0.f, 0.f, 0.f};
             {
                 const int t = (lane & 7) + 8 * ((lane >> 4) & 1);
                 const uint32_t a0 = kbase + t * ROW_PITCH + 16 * ((lane >> 3) & 1);
@@ -215,9 +217,13 @@ __global__ void __launch_bounds__(WARPS * 32) row_attn_kernel(const RowAttnParam
                 for (int ks = 0; ks < 8; ++ks) {
                     uint32_t kb[4];
                     ldmatrix_x4(kb, a0 + 32 * ks);
-                    mma_bf16_k16(s0, qa[ks][0], qa[ks][1], qa[ks][2], qa[ks][3], kb[0], kb[1]);
-                    mma_bf16_k16(s1, qa[ks][0], qa[ks][1], qa[ks][2], qa[ks][3], kb[2], kb[3]);
+                    mma_bf16_k16(ks & 1 ? u0 : s0, qa[ks][0], qa[ks][1], qa[ks][2], qa[ks][3],
+                                 kb[0], kb[1]);
+                    mma_bf16_k16(ks & 1 ? u1 : s1, qa[ks][0], qa[ks][1], qa[ks][2], qa[ks][3],
+                                 kb[2], kb[3]);
                 }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) { s0[i] += u0[i]; s1[i] += u1[i]; }
             }
             // scores in units of log2; x[0..3] row a, x[4..7] row b, keys 2 tig,
             // 2 tig + 1, 2 tig + 8, 2 tig + 9 of the page
@@ -250,10 +256,14 @@ __global__ void __launch_bounds__(WARPS * 32) row_attn_kernel(const RowAttnParam
             float al_b = 1.f;
             if (HI) al_b = softmax4(x + 4, m_b, l_b);
             else x[4] = x[5] = x[6] = x[7] = 0.f;
+            if (!HI) al_b = al_a;
+            // (the maximum of most pages is not a new one)
+            if (__any_sync(0xffffffffu, al_a != 1.f || al_b != 1.f)) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                acc[i][0] *= al_a; acc[i][1] *= al_a;
-                if (HI) { acc[i][2] *= al_b; acc[i][3] *= al_b; }
+                for (int i = 0; i < 16; ++i) {
+                    acc[i][0] *= al_a; acc[i][1] *= al_a;
+                    acc[i][2] *= al_b; acc[i][3] *= al_b;
+                }
             }
             uint32_t ph[4], pl[4];
 #pragma unroll
@@ -270,15 +280,24 @@ __global__ void __launch_bounds__(WARPS * 32) row_attn_kernel(const RowAttnParam
                 for (int dp = 0; dp < 8; ++dp) {
                     uint32_t vb[4];
                     ldmatrix_x4_trans(vb, a0 + 32 * dp);
-                    mma_bf16_k16(acc[2 * dp], ph[0], ph[1], ph[2], ph[3], vb[0], vb[1]);
-                    mma_bf16_k16(acc[2 * dp + 1], ph[0], ph[1], ph[2], ph[3], vb[2], vb[3]);
-                    mma_bf16_k16(acc[2 * dp], pl[0], pl[1], pl[2], pl[3], vb[0], vb[1]);
-                    mma_bf16_k16(acc[2 * dp + 1], pl[0], pl[1], pl[2], pl[3], vb[2], vb[3]);
+                    if (HI) {
+                        mma_bf16_k16(acc[2 * dp], ph[0], ph[1], ph[2], ph[3], vb[0], vb[1]);
+                        mma_bf16_k16(acc[2 * dp + 1], ph[0], ph[1], ph[2], ph[3], vb[2], vb[3]);
+                        mma_bf16_k16(acc[2 * dp], pl[0], pl[1], pl[2], pl[3], vb[0], vb[1]);
+                        mma_bf16_k16(acc[2 * dp + 1], pl[0], pl[1], pl[2], pl[3], vb[2], vb[3]);
+                    } else {
+                        // up to 8 rows: the lower terms ride in fragment rows 8-15
+                        mma_bf16_k16(acc[2 * dp], ph[0], pl[0], ph[2], pl[2], vb[0], vb[1]);
+                        mma_bf16_k16(acc[2 * dp + 1], ph[0], pl[0], ph[2], pl[2], vb[2], vb[3]);
+                    }
                 }
             }
             __syncwarp();                       // the stage is free
         }
 
+        if (!HI)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) { acc[i][0] += acc[i][2]; acc[i][1] += acc[i][3]; }
         // ---- the warps of the CTA -------------------------------------------------
         l_a += __shfl_xor_sync(0xffffffffu, l_a, 1);
         l_a += __shfl_xor_sync(0xffffffffu, l_a, 2);
@@ -443,18 +462,18 @@ int launch_row(const char* who, const RowAttnParams& p, int n_req, cudaStream_t 
 
 int launch_row_attn(const char* who, const RowAttnParams& p, int n_req, int most_rows,
                     cudaStream_t s) {
-    // Small CTAs (four warps, three pages in flight each, two CTAs to an SM) once there
-    // are enough pairs for most SMs; clusters of eight-warp CTAs below.  64 requests x 8
-    // heads x 129 pages: 95 us (5.7 TB/s) against 120 with two pages in flight, three CTAs
-    // to an SM, 102 with two warps and 125 with eight-warp CTAs, one to an SM; 8 pairs x
-    // 257 pages: 10.3 us in clusters of eight.
+    // Small CTAs (four warps, three stages, two CTAs to an SM) once there are enough pairs
+    // for most SMs; clusters of eight-warp CTAs below.  64 requests x 8 heads x 129 pages:
+    // 87 us (6.2 TB/s); with two stages and three CTAs to an SM 120, with two warps 102,
+    // with eight-warp CTAs, one to an SM, 125.  8 pairs x 257 pages in clusters of eight:
+    // 9.6 us, with four-warp CTAs 10.5.
     const int64_t pairs = (int64_t)n_req * p.n_kv;
     const bool hi = most_rows > 8;
     if (2 * pairs > sm_count())
         return hi ? launch_row<4, 3, false, true>(who, p, n_req, s)
                   : launch_row<4, 3, false, false>(who, p, n_req, s);
-    return hi ? launch_row<8, 2, true, true>(who, p, n_req, s)
-              : launch_row<8, 2, true, false>(who, p, n_req, s);
+    return hi ? launch_row<8, 3, true, true>(who, p, n_req, s)
+              : launch_row<8, 3, true, false>(who, p, n_req, s);
 }
 
 }  // namespace locks
