@@ -145,6 +145,7 @@ struct TileAttnParams {
     float *parts_out, *parts_ml;
     int* status;
     int head_chunks;                  // 64-channel chunks between two heads
+    int tile_bound;                   // upper bound of the row tiles, 0: count them
 };
 
 // csrc/row_attn.cu; `who` names the entry point in error messages, no request has more

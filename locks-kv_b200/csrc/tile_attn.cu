@@ -199,8 +199,9 @@ struct FindState {
     int s0, before;
 };
 
-// Work item `w` of `total` tiles x KV heads x parts, tiles fastest, by one warp.
-__device__ __forceinline__ void find_item(const TileAttnParams& p, int w, int total, int lane,
+// Work item `w` of `total` tiles x KV heads x parts, tiles fastest, by one warp; false:
+// there is no such tile (total an upper bound).
+__device__ __forceinline__ bool find_item(const TileAttnParams& p, int w, int total, int lane,
                                           FindState& at, Item& it) {
     const int target = w % total, rest = w / total;
     if (target < at.before) at = {0, 0};
@@ -255,10 +256,11 @@ __device__ __forceinline__ void find_item(const TileAttnParams& p, int w, int to
             it.j0 = min(it.part * per, all);
             it.n_tiles = min(it.j0 + per, all) - it.j0;
             it.valid = 1;
-            return;
+            return true;
         }
         at.before += __shfl_sync(0xffffffffu, x, 31);
     }
+    return false;
 }
 
 __global__ void __launch_bounds__(TA_THREADS, 1)
@@ -316,13 +318,14 @@ tile_attn_kernel(const __grid_constant__ CUtensorMap map_q,
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
         if (warp == 10) {
             // ---- items ----------------------------------------------------------------
-            const int tiles = count_tiles(p, lane), total = tiles * p.r.n_kv * p.parts;
+            const int tiles = p.tile_bound ? p.tile_bound : count_tiles(p, lane);
+            const int total = tiles * p.r.n_kv * p.parts;
             FindState at = {0, 0};
             int n = 0;
             for (int w = blockIdx.x; !__any_sync(0xffffffffu, is_dead(sm)); w += gridDim.x) {
                 Item it;
                 it.valid = 0;
-                if (w < total) find_item(p, w, tiles, lane, at, it);
+                if (w < total && !find_item(p, w, tiles, lane, at, it)) continue;
                 if (n >= 2)
                     ta_wait(sm, &sm.item_empty[n & 1], (uint32_t)((n >> 1) - 1) & 1u, p.status);
                 if (lane == 0) {
@@ -931,6 +934,8 @@ int launch_tile_attn(const char* who, TileAttnParams p, int max_tiles, int n_tok
     }
     const int64_t items = (int64_t)max_tiles * p.r.n_kv * p.parts;
     LOCKS_REQUIRE(items < (1 << 30), LOCKS_ERR_SIZE, "%s: too many query rows in one call", who);
+    // (with a CTA for every tile there could be, nobody has to count them first)
+    p.tile_bound = items <= sm_count() ? max_tiles : 0;
     tile_attn_kernel<<<(int)(items < sm_count() ? items : sm_count()), TA_THREADS, smem, s>>>(
         mq, mk, mv, p);
     return check_launch(who);
