@@ -627,8 +627,10 @@ int locks_dense_decode(const void* q, int64_t q_stride_req, const void* k_cache,
  * query runs with the last row of q (n_tok).  scale must be positive.
  * lse: optional f32 natural log-sum-exp, lse[token * lse_stride_tok + head].
  * max_q: no request has more query tokens (a bound the host knows).
- * scratch: optional fp32 workspace; what the call leaves there is of no use to
- * anyone, and calls that may overlap on the GPU need one each.
+ * scratch: optional fp32 workspace of scratch_floats elements, for cutting long keys
+ * of few queries into parts of n_tok * n_kv * G * (head_dim + 2) elements each (as
+ * many as fit, none below two); what the call leaves there is of no use to anyone,
+ * and calls that may overlap on the GPU need one each.
  *
  * locks_shared_prefix_decode: one query token per request (row r of q, position
  * seq_lens[r] - 1), requests [cu_groups[g], cu_groups[g + 1]) share the first

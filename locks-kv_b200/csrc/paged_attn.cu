@@ -37,6 +37,11 @@ int check_paged(const char* who, const RowAttnParams& p, int n_req, int head_dim
 // fragments hold 16; above it the tiled kernel takes 128 rows at a time.
 constexpr int FEW_ROWS = 16;
 constexpr int TILE_ROWS = 256, TILE_PAGES = 8;
+// Few (request, KV head) pairs whose lists may be this long are worth more CTAs than a
+// cluster has, and a launch that joins their parts (3 us).  8 pairs, in clusters and in
+// parts: 2048 pages 36 and 32 us, 4096 pages 64 and 53, 8192 pages 122 and 96; 2 pairs x
+// 8192 pages 87 and 46.
+constexpr int LONG_PAGES = 2048;
 
 // How many parts the key tiles are cut into: enough CTAs for the device, at least two
 // tiles a part (one per stream), as many as the scratch has room for.
@@ -83,6 +88,10 @@ extern "C" int locks_window_attention(
     if (n_req == 0 || n_tok == 0 || max_q == 0) return LOCKS_OK;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     p.max_rows = INT32_MAX;
+    const int64_t span = (int64_t)window + sinks + max_q;
+    const int64_t pages = span / page + 2 < bt_width ? span / page + 2 : bt_width;
+    TileAttnParams tp = {};
+    tp.part_rows = (int64_t)n_tok * n_kv * G;
     if ((int64_t)max_q * G > FEW_ROWS) {
         // (how the tokens fall on the requests is known on the device only: an upper
         // bound of the tiles, CTAs without one return at once)
@@ -92,13 +101,9 @@ extern "C" int locks_window_attention(
         const int64_t most = many * (((int64_t)max_q * G + TILE_ROWS - 1) / TILE_ROWS);
         tiles = tiles < most ? tiles : most;
         if (tiles > 0) {
-            TileAttnParams tp = {};
+            p.max_rows = FEW_ROWS;
             tp.r = p;
             tp.bounds = cu_q; tp.n_seg = n_req; tp.min_rows = FEW_ROWS; tp.status = status;
-            const int64_t span = (int64_t)window + sinks + max_q;
-            const int64_t pages = span / page + 2 < bt_width ? span / page + 2 : bt_width;
-            p.max_rows = FEW_ROWS;
-            tp.part_rows = (int64_t)n_tok * n_kv * G;
             tp.parts = scratch ? parts_for(tiles * n_kv, pages, tp.part_rows * (PR_HD + 2),
                                            scratch_floats) : 1;
             if (tp.parts > 1) {
@@ -108,12 +113,26 @@ extern "C" int locks_window_attention(
             p.beside = 1;
             int rc2 = launch_tile_attn(who, tp, (int)tiles, n_tok, s);
             if (rc2 == LOCKS_OK)
-                rc2 = launch_row_attn(who, p, n_req, max_q < FEW_ROWS ? max_q * G : FEW_ROWS, s);
+                rc2 = launch_row_attn(who, p, n_req, max_q < FEW_ROWS ? max_q * G : FEW_ROWS, 1,
+                                      s);
             if (rc2 == LOCKS_OK && tp.parts > 1) rc2 = launch_join_parts(who, tp, tp.parts, n_tok, s);
             return rc2;
         }
     }
-    return launch_row_attn(who, p, n_req, max_q < FEW_ROWS ? max_q * G : FEW_ROWS, s);
+    const int64_t pairs = (int64_t)n_req * n_kv;
+    int64_t splits = scratch ? scratch_floats / (tp.part_rows * (PR_HD + 2)) : 0;
+    splits = splits < 2 * sm_count() / pairs ? splits : 2 * sm_count() / pairs;
+    if (pages < LONG_PAGES || splits < 4)
+        return launch_row_attn(who, p, n_req, max_q < FEW_ROWS ? max_q * G : FEW_ROWS, 1, s);
+    p.part_rows = tp.part_rows;
+    p.parts_o = scratch;
+    p.parts_ml = scratch + splits * tp.part_rows * PR_HD;
+    tp.r = p;
+    tp.bounds = cu_q; tp.n_seg = n_req; tp.min_rows = -1;       // (no tiles: all rows joined)
+    tp.parts_out = p.parts_o; tp.parts_ml = p.parts_ml;
+    const int rc2 = launch_row_attn(
+        who, p, n_req, max_q < FEW_ROWS ? max_q * G : FEW_ROWS, (int)splits, s);
+    return rc2 == LOCKS_OK ? launch_join_parts(who, tp, (int)splits, n_tok, s) : rc2;
 }
 
 extern "C" int locks_shared_prefix_decode(
@@ -168,7 +187,7 @@ extern "C" int locks_shared_prefix_decode(
     p.part = tp.parts; p.part_rows = tp.part_rows;
     p.parts_o = tp.parts_out; p.parts_ml = tp.parts_ml;
     int rc2 = launch_tile_attn(who, tp, (int)tiles, n_req, s);
-    if (rc2 == LOCKS_OK) rc2 = launch_row_attn(who, p, n_req, G, s);
+    if (rc2 == LOCKS_OK) rc2 = launch_row_attn(who, p, n_req, G, 1, s);
     if (rc2 == LOCKS_OK) rc2 = launch_join_parts(who, tp, tp.parts + 1, n_req, s);
     return rc2;
 }

@@ -149,9 +149,10 @@ struct TileAttnParams {
 };
 
 // csrc/row_attn.cu; `who` names the entry point in error messages, no request has more
-// than most_rows rows that the launch has to serve
+// than most_rows rows that the launch has to serve.  splits > 1: that many CTAs to a pair,
+// whose results become parts p.part ..
 int launch_row_attn(const char* who, const RowAttnParams& p, int n_req, int most_rows,
-                    cudaStream_t s);
+                    int splits, cudaStream_t s);
 // csrc/tile_attn.cu
 int launch_tile_attn(const char* who, TileAttnParams p, int max_tiles, int n_tok,
                      cudaStream_t s);

@@ -21,7 +21,9 @@
 //                                   start and end overlap the others' pages;
 //   few                             a thread-block cluster each: its CTAs push (m, l, O)
 //                                   into each other's shared memory and finish a slice
-//                                   of the output each -- no partials in HBM, one launch.
+//                                   of the output each -- no partials in HBM, one launch;
+//   few, very long lists            the small CTAs again, many to a pair, their results
+//                                   joined by a launch behind them.
 //
 // P is split into two bf16 terms (P = hi + lo to 2^-17), so the product with V
 // loses nothing to P's rounding; with up to 8 rows both terms share one product, above
@@ -84,7 +86,7 @@ __global__ void __launch_bounds__(WARPS * 32) row_attn_kernel(const RowAttnParam
     using Smem = RowSmem<WARPS, STAGES, CLUSTER>;
     Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
     constexpr int THREADS = WARPS * 32;
-    const int c = CLUSTER ? blockIdx.x : 0, CL = CLUSTER ? gridDim.x : 1;
+    const int c = blockIdx.x, CL = gridDim.x;    // the pair's CTA, of how many
     const int kh = blockIdx.y, r = blockIdx.z;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int gid = lane >> 2, tig = lane & 3;
@@ -342,8 +344,9 @@ __global__ void __launch_bounds__(WARPS * 32) row_attn_kernel(const RowAttnParam
         auto finish = [&](int row, int d, float M, float L, float4 o) {
             const int at = rb * 16 + row, i = at / G, h = kh * G + at - i * G;
             if (p.parts_o) {
-                // one of several parts (one query token per request: i == 0, tok0 == r)
-                const int64_t x = p.part * p.part_rows + (int64_t)tok0 * p.n_kv * G + h;
+                // one of several parts
+                const int64_t x = (p.part + (CLUSTER ? 0 : c)) * p.part_rows +
+                                  (int64_t)(tok0 + i) * p.n_kv * G + h;
                 *reinterpret_cast<float4*>(p.parts_o + x * PR_HD + d) = o;
                 if (d == 0)
                     *reinterpret_cast<float2*>(p.parts_ml + 2 * x) = make_float2(M, L);
@@ -405,7 +408,8 @@ __global__ void __launch_bounds__(WARPS * 32) row_attn_kernel(const RowAttnParam
 }
 
 template <int WARPS, int STAGES, bool CLUSTER, bool HI>
-int launch_row(const char* who, const RowAttnParams& p, int n_req, cudaStream_t s) {
+int launch_row(const char* who, const RowAttnParams& p, int n_req, int splits,
+               cudaStream_t s) {
     auto kernel = row_attn_kernel<WARPS, STAGES, CLUSTER, HI>;
     // clusters of 2, 4, 8 and 16 CTAs the device holds at once (a cluster lives in one
     // GPC, so that fewer of the large ones fit than SMs would suggest)
@@ -424,7 +428,7 @@ int launch_row(const char* who, const RowAttnParams& p, int n_req, cudaStream_t 
         }
         attr_done[dev] = true;
     }
-    int cl = 1;
+    int cl = splits;
     if (CLUSTER) {
         // the largest that lets every pair's cluster run at once
         cl = 2;
@@ -461,7 +465,7 @@ int launch_row(const char* who, const RowAttnParams& p, int n_req, cudaStream_t 
 }  // namespace
 
 int launch_row_attn(const char* who, const RowAttnParams& p, int n_req, int most_rows,
-                    cudaStream_t s) {
+                    int splits, cudaStream_t s) {
     // Small CTAs (four warps, three stages, two CTAs to an SM) once there are enough pairs
     // for most SMs; clusters of eight-warp CTAs below.  64 requests x 8 heads x 129 pages:
     // 87 us (6.2 TB/s); with two stages and three CTAs to an SM 120, with two warps 102,
@@ -469,11 +473,11 @@ int launch_row_attn(const char* who, const RowAttnParams& p, int n_req, int most
     // 9.6 us, with four-warp CTAs 10.5.
     const int64_t pairs = (int64_t)n_req * p.n_kv;
     const bool hi = most_rows > 8;
-    if (2 * pairs > sm_count())
-        return hi ? launch_row<4, 3, false, true>(who, p, n_req, s)
-                  : launch_row<4, 3, false, false>(who, p, n_req, s);
-    return hi ? launch_row<8, 3, true, true>(who, p, n_req, s)
-              : launch_row<8, 3, true, false>(who, p, n_req, s);
+    if (2 * pairs > sm_count() || splits > 1)
+        return hi ? launch_row<4, 3, false, true>(who, p, n_req, splits, s)
+                  : launch_row<4, 3, false, false>(who, p, n_req, splits, s);
+    return hi ? launch_row<8, 3, true, true>(who, p, n_req, 1, s)
+              : launch_row<8, 3, true, false>(who, p, n_req, 1, s);
 }
 
 }  // namespace locks

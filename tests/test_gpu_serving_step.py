@@ -218,6 +218,8 @@ WINDOW_CASES = [
     (1, 4, [(1000, 1100)], 128, 0),
     (1, 8, [(40, 17000)], None, 0),
     (1, 1, [(130, 6000), (300, 300)], 5000, 1000),
+    (1, 8, [(1, 40001), (2, 33000), (0, 7), (1, 3)], None, 0),   # few rows, very long
+    (2, 16, [(1, 36000)], 34000, 50),
 ]
 
 
