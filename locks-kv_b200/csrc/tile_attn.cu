@@ -30,8 +30,9 @@
 // Tensor memory: S / P of the streams in columns 0 and 128, O in 256 and 384.
 //
 // The running maximum is only raised when it grows by more than 2^8 (O and l then get
-// rescaled): P stays below 2^8 and no row of O is touched in most steps.  P is rounded to bf16 because V is (both operands of the
-// product have one type), half a step each; m, l, S and O are fp32.
+// rescaled): P stays below 2^8 and no row of O is touched in most steps.  P is rounded to
+// bf16 because V is (both operands of the product have one type), half a step each; m, l,
+// S and O are fp32.
 //
 // Every wait is bounded (status word; later waits then return at once, work and copies
 // in flight are waited for and tensor memory is freed).  No multicast.
@@ -59,7 +60,7 @@ constexpr int TA_POLY = 4;
 constexpr int TA_EARLY = 4;                        // pages (k-steps) of the first step
 
 struct Item {
-    int valid, seg, kh, part, t0, row0, n_rows, j0, n_tiles, key_end, written, base_pos;
+    int valid, kh, part, t0, row0, n_rows, j0, n_tiles, key_end, written, base_pos;
     int table_row;
     PageList list;
 };
@@ -70,7 +71,7 @@ struct __align__(1024) TileSmem {
     uint8_t stage[8][4096];                        // a softmax warp's way out: 32 rows x 128 B
     uint64_t full[TA_RING], empty[TA_RING], tail, drain;
     uint64_t item_full[2], item_empty[2], q_full[2], q_empty;
-    uint64_t s_full[2], p_early[2], p_ready[2], o_full[2];
+    uint64_t s_full[2], p_early[2], p_ready[2], o_full[2], meet;
     Item item[2];
     uint32_t tmem_base;
     int dead;
@@ -224,7 +225,6 @@ __device__ __forceinline__ bool find_item(const TileAttnParams& p, int w, int to
         const uint32_t hit = __ballot_sync(0xffffffffu, target >= from && target < from + mine);
         if (hit) {
             const int src = __ffs(hit) - 1;
-            it.seg = s0 + src;
             it.t0 = __shfl_sync(0xffffffffu, t0, src);
             n = __shfl_sync(0xffffffffu, n, src);
             extent = __shfl_sync(0xffffffffu, extent, src);
@@ -245,7 +245,7 @@ __device__ __forceinline__ bool find_item(const TileAttnParams& p, int w, int to
                 it.written = extent;
                 // (where the queries sit goes by the bounds, cut off or not)
                 it.base_pos = it.written - (__shfl_sync(0xffffffffu, end, src) - it.t0);
-                it.table_row = it.seg;
+                it.table_row = s0 + src;
                 it.list = page_list(it.base_pos + it.row0 / G,
                                     it.base_pos + (it.row0 + it.n_rows - 1) / G, p.r.window,
                                     p.r.sinks, p.r.bt_width);
@@ -279,6 +279,7 @@ tile_attn_kernel(const __grid_constant__ CUtensorMap map_q,
         for (int i = 0; i < TA_RING; ++i) { mbar_init(&sm.full[i], 1); mbar_init(&sm.empty[i], 1); }
         mbar_init(&sm.tail, 1);
         mbar_init(&sm.drain, 1);
+        mbar_init(&sm.meet, 8);
         mbar_init(&sm.q_empty, 1);
         for (int i = 0; i < 2; ++i) {
             mbar_init(&sm.item_full[i], 1);
@@ -583,6 +584,12 @@ tile_attn_kernel(const __grid_constant__ CUtensorMap map_q,
         const uint32_t ts = lane_base + TM_S + i * TA_TILE;
         const float sl2 = p.r.scale_log2;
         uint32_t phase = 0;                         // tiles of this stream, over all items
+        uint32_t meetings = 0;
+        auto meet = [&]() {                         // all eight softmax warps (bounded too)
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sm.meet);
+            ta_wait(sm, &sm.meet, meetings++ & 1u, p.status);
+        };
         for (int n = 0;; ++n) {
             const Item* item = next_item(n);
             if (!item) break;
@@ -731,10 +738,10 @@ tile_attn_kernel(const __grid_constant__ CUtensorMap map_q,
                 float2* mine = reinterpret_cast<float2*>(sm.stage[warp]) + lane;
                 *mine = make_float2(m, l);
                 tc_before_sync();
-                asm volatile("bar.sync 1, 256;" ::: "memory");
+                meet();
                 tc_after_sync();
                 const float2 other = reinterpret_cast<float2*>(sm.stage[warp ^ 4])[lane];
-                asm volatile("bar.sync 1, 256;" ::: "memory");
+                meet();
                 const float m1 = other.x, l1 = other.y;
                 const float up = fmaxf(m, m1);
                 w_mine = l > 0.f ? pr_exp2((m - up) * sl2) : 0.f;
@@ -833,7 +840,7 @@ tile_attn_kernel(const __grid_constant__ CUtensorMap map_q,
             }
             tc_before_sync();
             // (the other stream has read this one's O and sums before they change)
-            if (!by_rows) asm volatile("bar.sync 1, 256;" ::: "memory");
+            if (!by_rows) meet();
         }
     }
     __syncwarp();
