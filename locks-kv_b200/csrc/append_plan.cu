@@ -30,8 +30,7 @@ namespace cg = cooperative_groups;
 namespace locks {
 namespace {
 
-constexpr int AP_THREADS = 1024;
-constexpr int AP_WARPS = AP_THREADS / 32;
+constexpr int AP_FEW = 128, AP_MANY = 1024;      // threads of a CTA: small steps, large ones
 constexpr int AP_MAX_REQS = 4096;
 constexpr int AP_MAX_CL = 16;
 
@@ -53,6 +52,7 @@ struct PlanParams {
 
 // exclusive prefix sum of one value per thread over the block; `total` on every
 // thread.  Two barriers.
+template <int THREADS>
 __device__ __forceinline__ int block_excl_scan(int v, int* sh, int& total) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     int x = v;
@@ -67,7 +67,7 @@ __device__ __forceinline__ int block_excl_scan(int v, int* sh, int& total) {
     int before = 0;
     total = 0;
 #pragma unroll
-    for (int w = 0; w < AP_WARPS; ++w) {
+    for (int w = 0; w < THREADS / 32; ++w) {
         const int s = sh[w];
         if (w < warp) before += s;
         total += s;
@@ -79,15 +79,16 @@ __device__ __forceinline__ int pages_of(int tokens, int page) {
     return (int)(((int64_t)tokens + page - 1) / page);
 }
 
-__global__ void __launch_bounds__(AP_THREADS) append_plan_kernel(const PlanParams p) {
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS) append_plan_kernel(const PlanParams p) {
     extern __shared__ int sh_dyn[];
     int* s_cu = sh_dyn;                          // n_req + 1
     int* s_len = s_cu + p.n_req + 1;             // n_req
     int* s_first = s_len + p.n_req;              // n_req: first free index, -1 refused
-    __shared__ int sh[AP_WARPS];
+    __shared__ int sh[THREADS / 32];
     __shared__ int s_taken_max, s_refused;
     const int tid = threadIdx.x, rank = blockIdx.x, CL = gridDim.x;
-    const int per = (p.n_req + AP_THREADS - 1) / AP_THREADS;
+    const int per = (p.n_req + THREADS - 1) / THREADS;
     const int r0 = min(tid * per, p.n_req), r1 = min(r0 + per, p.n_req);
     if (tid == 0) { s_taken_max = 0; s_refused = 0; }
 
@@ -99,7 +100,7 @@ __global__ void __launch_bounds__(AP_THREADS) append_plan_kernel(const PlanParam
         n += s_cu[r];
     }
     int total;
-    int run = block_excl_scan(n, sh, total);
+    int run = block_excl_scan<THREADS>(n, sh, total);
     for (int r = r0; r < r1; ++r) {
         const int c = s_cu[r];
         s_cu[r] = run;
@@ -119,7 +120,7 @@ __global__ void __launch_bounds__(AP_THREADS) append_plan_kernel(const PlanParam
     bool fits;
     for (int r = r0; r < r1; ++r) need += need_of(r, fits);
     int all_need;
-    int upto = block_excl_scan(need, sh, all_need);
+    int upto = block_excl_scan<THREADS>(need, sh, all_need);
     int my_max = 0;
     bool refused = false;
     for (int r = r0; r < r1; ++r) {
@@ -137,7 +138,7 @@ __global__ void __launch_bounds__(AP_THREADS) append_plan_kernel(const PlanParam
 
     // ---- outputs ----------------------------------------------------------------
     if (rank == 0) {
-        for (int r = tid; r < p.n_req; r += AP_THREADS) {
+        for (int r = tid; r < p.n_req; r += THREADS) {
             p.cu[r] = s_cu[r];
             p.lens_out[r] = s_len[r] + (s_first[r] >= 0 ? s_cu[r + 1] - s_cu[r] : 0);
         }
@@ -147,7 +148,7 @@ __global__ void __launch_bounds__(AP_THREADS) append_plan_kernel(const PlanParam
             if (s_refused && p.status) atomicExch(p.status, LOCKS_ST_PLAN_REFUSED);
         }
     }
-    for (int t = rank * AP_THREADS + tid; t < p.cap; t += CL * AP_THREADS) {
+    for (int t = rank * THREADS + tid; t < p.cap; t += CL * THREADS) {
         if (t >= total) { p.slot[t] = -1; p.pos[t] = 0; continue; }
         int lo = 0, hi = p.n_req - 1;            // the request with cu[r] <= t < cu[r+1]
         while (lo < hi) {
@@ -194,23 +195,28 @@ extern "C" int locks_append_plan(const int32_t* seq_lens, const int32_t* n_new,
     p.slot = slot_mapping; p.pos = positions; p.cu = cu_tokens;
     p.lens_out = lens_out; p.taken_out = taken_out;
     p.status = status; p.n_req = n_req; p.cap = max_tokens; p.page = page;
+    // 16 requests, one token each: 3.7 us with 128 threads, 5.5 with 1024; 256 requests,
+    // 65536 tokens: 11 us with 16 CTAs of 1024, 20 with 8 of 512
+    const bool few = n_req <= 2 * AP_FEW && max_tokens <= 4 * AP_FEW;
+    void (*kernel)(const PlanParams) =
+        few ? append_plan_kernel<AP_FEW> : append_plan_kernel<AP_MANY>;
     const int smem = (3 * n_req + 1) * (int)sizeof(int);
     static bool attr_done[64] = {false};
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev >= 0 && dev < 64 && !attr_done[dev]) {
-        cudaFuncSetAttribute(append_plan_kernel,
+        cudaFuncSetAttribute(append_plan_kernel<AP_MANY>,
                              cudaFuncAttributeMaxDynamicSharedMemorySize,
                              (3 * AP_MAX_REQS + 1) * (int)sizeof(int));
-        cudaFuncSetAttribute(append_plan_kernel,
+        cudaFuncSetAttribute(append_plan_kernel<AP_MANY>,
                              cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         attr_done[dev] = true;
     }
     int cl = 1;
-    while (cl < AP_MAX_CL && cl * AP_THREADS < max_tokens) cl *= 2;
+    while (!few && cl < AP_MAX_CL && cl * AP_MANY < max_tokens) cl *= 2;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(cl, 1, 1);
-    cfg.blockDim = dim3(AP_THREADS, 1, 1);
+    cfg.blockDim = dim3(few ? AP_FEW : AP_MANY, 1, 1);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = static_cast<cudaStream_t>(stream);
     cudaLaunchAttribute attr[1];
@@ -220,7 +226,7 @@ extern "C" int locks_append_plan(const int32_t* seq_lens, const int32_t* n_new,
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, append_plan_kernel, p);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
     if (e != cudaSuccess)
         return fail(LOCKS_ERR_LAUNCH, "locks_append_plan: %s", cudaGetErrorString(e));
     pdl_break();             // the scorer reads block tables before its wait

@@ -60,9 +60,10 @@ def window_paged_attention(q: torch.Tensor, kv_cache: torch.Tensor,
     position p sees keys j <= p with p - j < ``window`` or j < ``sinks``
     (``window`` None: all of them).  Rows that see nothing become 0 (lse -inf),
     rows behind ``cu_q[R]`` stay as they were, pages that nobody sees are not read.
-    ``max_q`` bounds the query tokens of a request.  ``scratch``: fp32 workspace
-    for long keys with few queries, see :func:`attention_scratch_floats`; calls
-    that may overlap on the GPU need one each."""
+    ``max_q`` bounds the query tokens of a request (rows of one with more may be
+    left out).  ``scratch``: fp32 workspace that lets the long keys of few queries be
+    cut into parts, see :func:`attention_scratch_floats`; calls that may overlap on
+    the GPU need one each.  ``status``: int32, set where a bounded wait ran out."""
     dev = _cabi.one_device(q, kv_cache, block_table, cu_q, seq_lens, out, scratch, lse,
                            status)
     source, target, d, page = _checked(q, kv_cache, block_table, out, lse, scratch,
@@ -108,5 +109,6 @@ def attention_scratch_floats(n_rows: int, n_heads: int, head_dim: int = 128,
                              parts: int = 2) -> int:
     """fp32 elements that ``parts`` partial results of ``n_rows`` query tokens take
     (a maximum, a sum and ``head_dim`` values per head).  Shared-prefix decode needs
-    two, and uses up to one per 1 / (KV heads) of the device's SMs and one more."""
+    two; up to SMs / n_kv + 1 of them are of use to it, and up to 2 * SMs / (requests
+    * n_kv) to a windowed call with few queries over long keys."""
     return int(n_rows) * int(n_heads) * (int(head_dim) + 2) * int(parts)
