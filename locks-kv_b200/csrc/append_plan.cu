@@ -91,6 +91,7 @@ __global__ void __launch_bounds__(THREADS) append_plan_kernel(const PlanParams p
     const int per = (p.n_req + THREADS - 1) / THREADS;
     const int r0 = min(tid * per, p.n_req), r1 = min(r0 + per, p.n_req);
     if (tid == 0) { s_taken_max = 0; s_refused = 0; }
+    pdl_wait();                                  // (the lengths may be the last launch's)
 
     // ---- tokens -----------------------------------------------------------------
     int n = 0;
@@ -219,13 +220,15 @@ extern "C" int locks_append_plan(const int32_t* seq_lens, const int32_t* n_new,
     cfg.blockDim = dim3(few ? AP_FEW : AP_MANY, 1, 1);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = static_cast<cudaStream_t>(stream);
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = cl;
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = pdl_enabled() ? 2 : 1;
     const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
     if (e != cudaSuccess)
         return fail(LOCKS_ERR_LAUNCH, "locks_append_plan: %s", cudaGetErrorString(e));

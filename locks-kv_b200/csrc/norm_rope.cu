@@ -95,6 +95,9 @@ __global__ void __launch_bounds__(NR_THREADS, 8) norm_rope_kernel(const NormRope
     const int heads = p.H + 2 * p.n_kv, qk = p.H + p.n_kv;
     const int job = blockIdx.x * (NR_THREADS / 32) + (threadIdx.x >> 5);
     const int t = job / p.shares;
+    // launched behind the last kernel's end; the next one may line up once this one runs
+    pdl_wait();
+    pdl_trigger();
     if (t >= p.n_tok) return;                    // (a whole warp)
     const int h0 = (job - t * p.shares) * p.share;     // the warp's heads [h0, end)
     const int end = min(h0 + p.share, heads);
@@ -265,13 +268,22 @@ __global__ void __launch_bounds__(NR_THREADS, 8) norm_rope_kernel(const NormRope
 }
 
 template <class Tab>
-void launch_norm_rope(int mode, dim3 grid, cudaStream_t s, const NormRopeParams& p) {
-    switch (mode) {
-        case ROPE_NONE:   norm_rope_kernel<ROPE_NONE, Tab><<<grid, NR_THREADS, 0, s>>>(p); break;
-        case ROPE_PAIRS:  norm_rope_kernel<ROPE_PAIRS, Tab><<<grid, NR_THREADS, 0, s>>>(p); break;
-        case ROPE_HALVES: norm_rope_kernel<ROPE_HALVES, Tab><<<grid, NR_THREADS, 0, s>>>(p); break;
-        default:          norm_rope_kernel<ROPE_ANY, Tab><<<grid, NR_THREADS, 0, s>>>(p); break;
-    }
+cudaError_t launch_norm_rope(int mode, dim3 grid, cudaStream_t s, const NormRopeParams& p) {
+    void (*kernel)(const NormRopeParams) =
+        mode == ROPE_NONE ? norm_rope_kernel<ROPE_NONE, Tab>
+        : mode == ROPE_PAIRS ? norm_rope_kernel<ROPE_PAIRS, Tab>
+        : mode == ROPE_HALVES ? norm_rope_kernel<ROPE_HALVES, Tab>
+                              : norm_rope_kernel<ROPE_ANY, Tab>;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(NR_THREADS, 1, 1);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl_enabled() ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kernel, p);
 }
 
 bool rows16(const void* p, int64_t a, int64_t b) {
@@ -362,7 +374,9 @@ extern "C" int locks_norm_rope_write(
     p.shares = (steps + per - 1) / per;
     const dim3 grid((unsigned)(((int64_t)n_tok * p.shares + WARPS - 1) / WARPS), 1, 1);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (table_f32) launch_norm_rope<float>(mode, grid, s, p);
-    else launch_norm_rope<__nv_bfloat16>(mode, grid, s, p);
+    const cudaError_t e = table_f32 ? launch_norm_rope<float>(mode, grid, s, p)
+                                    : launch_norm_rope<__nv_bfloat16>(mode, grid, s, p);
+    if (e != cudaSuccess)
+        return fail(LOCKS_ERR_LAUNCH, "locks_norm_rope_write: %s", cudaGetErrorString(e));
     return check_launch("locks_norm_rope_write");
 }

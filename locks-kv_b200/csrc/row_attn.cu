@@ -91,6 +91,12 @@ __global__ void __launch_bounds__(WARPS * 32) row_attn_kernel(const RowAttnParam
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int gid = lane >> 2, tig = lane & 3;
     const int G = p.G;
+    // first launch of its call: everything before it on the stream is done, and the next
+    // launch may line up.  (Beside the tiled kernel that wait comes at the end.)
+    if (!p.beside) {
+        pdl_wait();
+        pdl_trigger();
+    }
     const int len = p.seq_lens[r];
     // shared prefix: the row's group, all bounds read at once; rows that belong to none
     // are left as they were
@@ -449,7 +455,7 @@ int launch_row(const char* who, const RowAttnParams& p, int n_req, int splits,
         attr[n].val.clusterDim.z = 1;
         ++n;
     }
-    if (p.beside && pdl_enabled()) {
+    if (pdl_enabled()) {
         attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
         attr[n].val.programmaticStreamSerializationAllowed = 1;
         ++n;

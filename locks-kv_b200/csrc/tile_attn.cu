@@ -298,7 +298,10 @@ tile_attn_kernel(const __grid_constant__ CUtensorMap map_q,
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
         tc_before_sync();
     }
-    pdl_trigger();                      // the call's next launch may take SMs as they free up
+    // everything before this launch is done; the call's next launch may take SMs as they
+    // free up
+    pdl_wait();
+    pdl_trigger();
     __syncthreads();
     tc_after_sync();
     const uint32_t tmem = sm.tmem_base;
@@ -943,8 +946,19 @@ int launch_tile_attn(const char* who, TileAttnParams p, int max_tiles, int n_tok
     LOCKS_REQUIRE(items < (1 << 30), LOCKS_ERR_SIZE, "%s: too many query rows in one call", who);
     // (with a CTA for every tile there could be, nobody has to count them first)
     p.tile_bound = items <= sm_count() ? max_tiles : 0;
-    tile_attn_kernel<<<(int)(items < sm_count() ? items : sm_count()), TA_THREADS, smem, s>>>(
-        mq, mk, mv, p);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(items < sm_count() ? items : sm_count()), 1, 1);
+    cfg.blockDim = dim3(TA_THREADS, 1, 1);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl_enabled() ? 1 : 0;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, tile_attn_kernel, mq, mk, mv, p);
+    if (e != cudaSuccess)
+        return fail(LOCKS_ERR_LAUNCH, "%s: %s", who, cudaGetErrorString(e));
     return check_launch(who);
 }
 
