@@ -613,7 +613,8 @@ int locks_dense_decode(const void* q, int64_t q_stride_req, const void* k_cache,
  * slot_mapping[t] (negative or beyond the cache: not stored).  fp32 throughout, one
  * rounding at the end.  Table and weights are bf16 or fp32 (table_f32, weight_f32);
  * weights have head_dim values.  Positions outside [0, n_positions) read the
- * nearest table row.  Two tokens with one slot leave either one's rows there.
+ * nearest table row.  Two tokens with one slot leave the rows of either there, head
+ * by head.
  *
  * locks_window_attention: attention of ragged query runs over the paged cache.
  * Request r's queries are tokens cu_q[r] .. cu_q[r + 1) of q; it has seq_lens[r]

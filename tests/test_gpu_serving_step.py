@@ -144,6 +144,24 @@ def test_norm_rope_odd_table_rows_and_outside_positions():
     assert used[:, 0].nonzero().tolist() == used[:, 1].nonzero().tolist() == [[0, 0], [1, 1], [2, 15]]
 
 
+def test_norm_rope_weight_on_one_side_only():
+    """A query weight alone leaves the keys unnormalised, and the other way round."""
+    from locks.attention import norm_rope_and_cache
+    g = torch.Generator(device=DEV).manual_seed(8)
+    q, k, v = (torch.randn(5, 2, 128, device=DEV, generator=g).to(BF16) for _ in range(3))
+    w = torch.rand(128, device=DEV, generator=g)
+    slots = torch.arange(5, device=DEV)
+    for kind in (torch.float32, BF16):
+        for wq, wk in ((w.to(kind), None), (None, w.to(kind))):
+            cache = torch.zeros(3, 2, 16, 2, 128, device=DEV, dtype=BF16)
+            out = norm_rope_and_cache(q, k, v, cache, slots, None, None, q_weight=wq, k_weight=wk,
+                                      eps=0.0, q_out=torch.empty_like(q))
+            for got, x, wt in ((out, q, wq), (cache[0, 0, :5], k, wk)):
+                want = ref.norm_rope(x, wt, 0.0, None, 0, True)
+                assert bool(((got.double() - want).abs() <= ref.HALF_BF16 * want.abs() + 1e-5).all())
+                assert wt is not None or torch.equal(got, x)
+
+
 # ---- paged inputs ---------------------------------------------------------------------
 def paged(seed, lens, n_kv, *, planes_first=False, spare=3):
     """A cache and tables of exactly the pages the lengths need, scattered."""
@@ -314,6 +332,24 @@ def test_window_head_major_cache_strided_table_and_no_programmatic_launch():
         _cabi.lib().locks_set_pdl(old)
     assert torch.equal(a, b)
     check(a[1:91], None, want_window(q[1:91], k, v, table[1], 300, 90, 100, 9))
+
+
+def test_block_ids_outside_the_cache_touch_nothing():
+    """Table entries of seen pages that name no block: read as some block of the cache,
+    never outside it; other requests are not affected."""
+    n_kv, G, reqs = 2, 8, [(1, 300), (60, 200), (1, 90), (40, 77)]
+    lens = [l for _, l in reqs]
+    g, cache, k, v, table = paged(31, lens, n_kv)
+    cu = [0, 1, 61, 62, 102]
+    table[0, ::2], table[1, 1::3] = -5, 2 ** 31 - 1
+    q = torch.randn(102, 16, 128, device=DEV, generator=g).to(BF16)
+    out = run_window(q, cache, table, i32(cu), i32(lens), n_kv, G, None, 0, 60)
+    assert bool(out.isfinite().all())
+    for r in (2, 3):
+        at = slice(cu[r], cu[r + 1])
+        check(out[at], None, want_window(q[at], k, v, table[r], lens[r], reqs[r][0], 2 ** 31 - 1, 0), r)
+    one = run_prefix(q[:4], cache, table, lens, [0, 2, 4], [64, 48], n_kv, G)
+    assert bool(one.isfinite().all())
 
 
 def test_offsets_beyond_31_bits():
