@@ -602,9 +602,9 @@ int locks_dense_decode(const void* q, int64_t q_stride_req, const void* k_cache,
  * the last token, up to max_tokens, become -1 / 0 (a padded batch).  A request that
  * does not fit -- its table row, the rest of the free list, or max_tokens -- is
  * refused as a whole: slots -1, no block, no entry, length unchanged, and *status
- * (optional) becomes LOCKS_ST_PLAN_REFUSED; later requests that fit are served
- * as long as they need no block the refused one left short.  n_req <= 4096; the sum
- * of n_new below 2^31.
+ * (optional) becomes LOCKS_ST_PLAN_REFUSED.  One refused for want of blocks ends the
+ * handing out: requests behind it are served if they need no block.  n_req <= 4096;
+ * bt_width * page and the sum of n_new below 2^31.
  *
  * locks_norm_rope_write: RMS norm of every query and key head (w / null: no norm),
  * rotation of the first rot_dim channels at positions[t] (null cos_sin: none;

@@ -185,7 +185,8 @@ extern "C" int locks_append_plan(const int32_t* seq_lens, const int32_t* n_new,
                       ((slot_mapping && positions) || max_tokens == 0),
                   LOCKS_ERR_ARG, "locks_append_plan: null pointer argument");
     LOCKS_REQUIRE(n_req >= 1 && bt_width >= 1 && bt_stride >= bt_width && n_free >= 0 &&
-                      max_tokens >= 0 && page >= 1,
+                      max_tokens >= 0 && page >= 1 &&
+                      (int64_t)bt_width * page <= INT32_MAX,
                   LOCKS_ERR_ARG, "locks_append_plan: bad size argument");
     LOCKS_REQUIRE(n_req <= AP_MAX_REQS, LOCKS_ERR_SIZE,
                   "locks_append_plan: at most %d requests, got %d", AP_MAX_REQS, n_req);

@@ -27,7 +27,8 @@ def append_plan(seq_lens: torch.Tensor, n_new: torch.Tensor,
     ``cu_tokens`` int32 (R + 1,), -1 / 0 behind the last token; ``lens_out`` int32
     (R,) and ``taken_out`` int32, one element (may be ``seq_lens`` and ``taken``
     themselves).  A request that does not fit its table row, the free list or T is
-    refused as a whole: slots -1, nothing else changed for it, ``status`` 3."""
+    refused as a whole: slots -1, nothing else changed for it, ``status`` 3; behind
+    one refused for want of blocks only requests that need none are served."""
     dev = _cabi.one_device(seq_lens, n_new, block_table, free_blocks, taken,
                            slot_mapping, positions, cu_tokens, lens_out, taken_out,
                            status)

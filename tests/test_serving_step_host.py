@@ -53,7 +53,7 @@ ODD = P((1 << 20) + 8)
 @pytest.mark.parametrize("change,code,word", [
     (dict(seq_lens=None), -1, "null"), (dict(free=None), -1, "null"), (dict(slots=None), -1, "null"),
     (dict(taken_out=None), -1, "null"), (dict(n_req=0), -1, "size"), (dict(bt_stride=7), -1, "size"),
-    (dict(page=0), -1, "size"), (dict(cap=-1), -1, "size"), (dict(n_req=4097), -4, "4096")])
+    (dict(page=0), -1, "size"), (dict(page=1 << 29), -1, "size"), (dict(cap=-1), -1, "size"), (dict(n_req=4097), -4, "4096")])
 def test_plan_refusals(change, code, word):
     got, msg = rc("locks_append_plan", with_(PLAN, **change))
     assert got == code and word in msg
