@@ -421,6 +421,55 @@ def test_window_repeats_bit_for_bit_on_another_stream():
     assert torch.equal(a, b)
 
 
+def test_calls_on_two_streams_at_once_and_two_graphs():
+    """Calls that overlap, each with a workspace of its own: what one after the other
+    gives, eagerly and from two graphs replayed side by side."""
+    n_kv, G, reqs = 2, 8, [(1, 700), (90, 400), (3, 2500)]
+    lens = [l for _, l in reqs]
+    cu = i32([0, 1, 91, 94])
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    calls, want = [], []
+    for k in range(2):
+        g, cache, _, _, table = paged(40 + k, lens, n_kv)
+        q = torch.randn(94, 16, 128, device=DEV, generator=g).to(BF16)
+        out, scratch = torch.empty_like(q), torch.empty(2 ** 20, device=DEV)
+        args = (q, cache, table, cu, i32(lens), n_kv, G, 200 + 300 * k, 4, 90)
+        calls.append((args, out, scratch))
+        want.append(run_window(*args, scratch=scratch).clone())
+    torch.cuda.synchronize()
+
+    def launch(k):
+        from locks.attention import window_paged_attention
+        (q, cache, table, cu_, ln, n, g_, w, s, mq), out, scratch = calls[k]
+        window_paged_attention(q, cache, table, cu_, ln, out, n_kv=n, G=g_, window=w, sinks=s,
+                               scale=SCALE, max_q=mq, scratch=scratch)
+
+    for _ in range(20):
+        for k in range(2):
+            calls[k][1].zero_()
+        torch.cuda.synchronize()
+        for k in range(2):
+            with torch.cuda.stream(streams[k]):
+                launch(k)
+        torch.cuda.synchronize()
+        assert all(torch.equal(calls[k][1], want[k]) for k in range(2))
+    graphs = []
+    for k in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[k]):
+            for _ in range(3):
+                launch(k)
+    for _ in range(10):
+        for k in range(2):
+            calls[k][1].zero_()
+        torch.cuda.synchronize()
+        for k in range(2):
+            with torch.cuda.stream(streams[k]):
+                graphs[k].replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(calls[k][1], want[k]) for k in range(2))
+
+
 # ---- shared prefix ----------------------------------------------------------------------
 def prefix_paged(seed, groups, n_kv, spare=3):
     """groups: [(prefix, [cached lengths])]; whole prefix pages shared, the page a
