@@ -158,6 +158,14 @@ rki4_score_kernel(const ScoreParams p) {
     const int kh = blockIdx.y;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     int z = blockIdx.x, Z = gridDim.x, r = blockIdx.z;
+    // A CTA without pages waits too: in a batch whose requests all lie inside their
+    // recent window no other one does, and the grid would end before the kernels in
+    // front of it -- the selector's and the decode's waits reach no further back than
+    // the launch before theirs.
+    auto leave = []() {
+        pdl_trigger();
+        pdl_wait();
+    };
     if (p.ragged) {
         // Ragged batch: the gridDim.x CTAs of a kv-head are dealt to the requests
         // in proportion to their chunk counts (every request gets one, the other
@@ -204,7 +212,10 @@ rki4_score_kernel(const ScoreParams p) {
             }
             acc += __shfl_sync(0xffffffffu, inc, 31);
         }
-        if (r < 0) return;                       // (no request: an empty batch)
+        if (r < 0) {                             // (no request: nothing to score)
+            leave();
+            return;
+        }
     }
     const int gid = lane >> 2, tig = lane & 3;
     const int G = p.G;
@@ -225,7 +236,10 @@ rki4_score_kernel(const ScoreParams p) {
     };
     const int blk0 = bt_at(gw * CHUNK), blk1 = bt_at((gw + W) * CHUNK);
     const int n_hi = min(p.n_sel_hi[r], cap);
-    if (n_hi <= 0) return;
+    if (n_hi <= 0) {
+        leave();
+        return;
+    }
     const int NC = (n_hi + CHUNK - 1) / CHUNK;
     const int n_items = (gw < NC) ? (NC - gw + W - 1) / W : 0;
     auto item_page0 = [&](int k) -> int { return (gw + k * W) * CHUNK; };

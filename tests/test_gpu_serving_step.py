@@ -663,3 +663,72 @@ def test_step_together_and_captured():
         torch.cuda.synchronize()
         expect([1, 1, 1])
     assert int(status) == 0
+
+
+@pytest.mark.parametrize("R", [1, 4])
+def test_norm_in_front_of_the_sparse_path_with_short_requests(R):
+    """Requests inside their recent window give the scorer nothing to do; the decode
+    behind it must still see the queries and the cache rows the head norm stores.  Two
+    layers over one set of selection buffers, eager and captured, the same bits as
+    without programmatic launches."""
+    from locks import _cabi
+    from locks.attention import norm_rope_and_cache, sparse_paged_decode_fused
+    from locks.config import LocksConfig
+    from locks.hotpath import HotPath
+    from locks.selection.rki4_score import rki4_score_state
+    L, n_kv, G, T = 2, 2, 4, 6000
+    H, lens = n_kv * G, [20, 33, 7, 48][:R]
+    g = torch.Generator(device=DEV).manual_seed(17)
+    base = [torch.randn(-(-T // 16) + 12, 2, 16, n_kv, 128, device=DEV, generator=g).to(BF16)
+            for _ in range(L)]
+    caches = [c.clone() for c in base]
+    table = torch.arange(1, 1 + 3 * R, device=DEV, dtype=I32).reshape(R, 3)
+    sl = i32(lens)
+    cfg = LocksConfig(budget_pages=2, sink_pages=1, window_pages=8)
+    hp = HotPath(caches, table, sl, n_kv=n_kv, G=G, scale=SCALE, cfg=cfg)
+    hp.derive()
+    assert bool((hp.st.n_sel_hi[:R] <= 0).all())
+    # a long norm launch whose last tokens are the requests' own
+    qkv = torch.randn(L, T, H + 2 * n_kv, 128, device=DEV, generator=g).to(BF16)
+    slots = torch.arange(T, device=DEV) + 13 * 16
+    slots[T - R:] = torch.tensor([int(table[r, (n - 1) // 16]) * 16 + (n - 1) % 16
+                                  for r, n in enumerate(lens)], device=DEV)
+    slots[T - R - 400:T - R] = -1
+    w = torch.rand(128, device=DEV, generator=g) + 0.5
+    qr, out = (torch.zeros(L, T, H, 128, device=DEV, dtype=BF16) for _ in range(2))
+
+    def step():
+        for l in range(L):
+            norm_rope_and_cache(qkv[l, :, :H], qkv[l, :, H:H + n_kv], qkv[l, :, H + n_kv:],
+                                caches[l], slots, None, None, q_weight=w, k_weight=w, q_out=qr[l])
+            q = qr[l, T - R:]
+            rki4_score_state(hp.st, l, q, table, sl, R, SCALE)
+            sparse_paged_decode_fused(q, caches[l], table, sl, hp.st, out[l, :R], hp.vsources[l])
+
+    def fresh(run):
+        qr.fill_(3.0)
+        out.fill_(float("nan"))
+        for c, b in zip(caches, base):
+            c.copy_(b)
+        torch.cuda.synchronize()
+        run()
+        torch.cuda.synchronize()
+        return out[:, :R].clone()
+
+    old = _cabi.lib().locks_set_pdl(0)
+    try:
+        want = fresh(step)
+    finally:
+        _cabi.lib().locks_set_pdl(old)
+    for l in range(L):
+        for r, n in enumerate(lens):
+            o, _, mean, _ = want_window(qr[l, T - R + r:T - R + r + 1], caches[l][:, 0], caches[l][:, 1],
+                                        table[r], n, 1, 2 ** 31 - 1, 0)
+            assert bool(((want[l, r:r + 1].double() - o).abs() <= 2e-2 + 1e-2 * mean).all())
+    for _ in range(10):
+        assert torch.equal(fresh(step), want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for _ in range(10):
+        assert torch.equal(fresh(graph.replay), want)
