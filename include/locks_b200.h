@@ -627,7 +627,9 @@ int locks_dense_decode(const void* q, int64_t q_stride_req, const void* k_cache,
  * Block ids are clamped to [0, num_blocks), keys end with the table's last column,
  * query runs with the last row of q (n_tok).  scale must be positive.
  * lse: optional f32 natural log-sum-exp, lse[token * lse_stride_tok + head].
- * max_q: no request has more query tokens (a bound the host knows).
+ * max_q: how many query tokens the longest request has.  It steers how the work is
+ * cut; a request with more is answered all the same, only more slowly (a captured
+ * call may meet one).  0: nothing is done.
  * scratch: optional fp32 workspace of scratch_floats elements, for cutting long keys
  * of few queries into parts of n_tok * n_kv * G * (head_dim + 2) elements each (as
  * many as fit, none below two); what the call leaves there is of no use to anyone,

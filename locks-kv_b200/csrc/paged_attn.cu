@@ -94,13 +94,14 @@ extern "C" int locks_window_attention(
     tp.part_rows = (int64_t)n_tok * n_kv * G;
     if ((int64_t)max_q * G > FEW_ROWS) {
         // (how the tokens fall on the requests is known on the device only: an upper
-        // bound of the tiles, CTAs without one return at once)
+        // bound of the tiles, CTAs without one return at once.  max_q may be too small:
+        // it lowers the count that is expected, not the bound)
         const int64_t rows = (int64_t)n_tok * G;
         const int64_t many = rows / (FEW_ROWS + 1) < n_req ? rows / (FEW_ROWS + 1) : n_req;
-        int64_t tiles = (rows + (TILE_ROWS - 1) * many) / TILE_ROWS;
+        const int64_t bound = (rows + (TILE_ROWS - 1) * many) / TILE_ROWS;
         const int64_t most = many * (((int64_t)max_q * G + TILE_ROWS - 1) / TILE_ROWS);
-        tiles = tiles < most ? tiles : most;
-        if (tiles > 0) {
+        const int64_t tiles = bound < most ? bound : most;
+        if (bound > 0) {
             p.max_rows = FEW_ROWS;
             tp.r = p;
             tp.bounds = cu_q; tp.n_seg = n_req; tp.min_rows = FEW_ROWS; tp.status = status;
@@ -111,7 +112,7 @@ extern "C" int locks_window_attention(
                 tp.parts_ml = scratch + tp.parts * tp.part_rows * PR_HD;
             }
             p.beside = 1;
-            int rc2 = launch_tile_attn(who, tp, (int)tiles, n_tok, s);
+            int rc2 = launch_tile_attn(who, tp, (int)tiles, (int)bound, n_tok, s);
             if (rc2 == LOCKS_OK)
                 rc2 = launch_row_attn(who, p, n_req, max_q < FEW_ROWS ? max_q * G : FEW_ROWS, 1,
                                       s);
@@ -186,7 +187,7 @@ extern "C" int locks_shared_prefix_decode(
     p.beside = 1;
     p.part = tp.parts; p.part_rows = tp.part_rows;
     p.parts_o = tp.parts_out; p.parts_ml = tp.parts_ml;
-    int rc2 = launch_tile_attn(who, tp, (int)tiles, n_req, s);
+    int rc2 = launch_tile_attn(who, tp, (int)tiles, (int)tiles, n_req, s);
     if (rc2 == LOCKS_OK) rc2 = launch_row_attn(who, p, n_req, G, 1, s);
     if (rc2 == LOCKS_OK) rc2 = launch_join_parts(who, tp, tp.parts + 1, n_req, s);
     return rc2;

@@ -145,16 +145,16 @@ struct TileAttnParams {
     float *parts_out, *parts_ml;
     int* status;
     int head_chunks;                  // 64-channel chunks between two heads
-    int tile_bound;                   // upper bound of the row tiles, 0: count them
+    int tile_bound, tile_more;        // row tiles expected and possible beyond; 0: count them
 };
 
-// csrc/row_attn.cu; `who` names the entry point in error messages, no request has more
-// than most_rows rows that the launch has to serve.  splits > 1: that many CTAs to a pair,
-// whose results become parts p.part ..
+// csrc/row_attn.cu; `who` names the entry point in error messages, most_rows: about how
+// many rows the longest request has that the launch serves (any number is served).
+// splits > 1: that many CTAs to a pair, whose results become parts p.part ..
 int launch_row_attn(const char* who, const RowAttnParams& p, int n_req, int most_rows,
                     int splits, cudaStream_t s);
-// csrc/tile_attn.cu
-int launch_tile_attn(const char* who, TileAttnParams p, int max_tiles, int n_tok,
+// csrc/tile_attn.cu; tiles: row tiles expected, max_tiles: there are no more than this
+int launch_tile_attn(const char* who, TileAttnParams p, int tiles, int max_tiles, int n_tok,
                      cudaStream_t s);
 int launch_join_parts(const char* who, const TileAttnParams& p, int parts, int n_tok,
                       cudaStream_t s);

@@ -79,13 +79,13 @@ __device__ __forceinline__ void axpy4(float4& o, float w, const float4 v) {
     o.z = fmaf(w, v.z, o.z); o.w = fmaf(w, v.w, o.w);
 }
 
-// HI: blocks may hold more than 8 rows
+// HI: rows are taken 16 to a block, else 8
 template <int WARPS, int STAGES, bool CLUSTER, bool HI>
 __global__ void __launch_bounds__(WARPS * 32) row_attn_kernel(const RowAttnParams p) {
     extern __shared__ __align__(128) uint8_t smem_raw[];
     using Smem = RowSmem<WARPS, STAGES, CLUSTER>;
     Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
-    constexpr int THREADS = WARPS * 32;
+    constexpr int THREADS = WARPS * 32, BLOCK = HI ? 16 : 8;
     const int c = blockIdx.x, CL = gridDim.x;    // the pair's CTA, of how many
     const int kh = blockIdx.y, r = blockIdx.z;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -127,9 +127,9 @@ __global__ void __launch_bounds__(WARPS * 32) row_attn_kernel(const RowAttnParam
     const int32_t* table = p.table + (int64_t)r * p.bt_stride;
 
     // (the loop bound is the same for every CTA of the cluster)
-    for (int rb = 0; rb * 16 < rows; ++rb) {
-        const int row_a = rb * 16 + gid, row_b = row_a + 8;
-        const int i_first = rb * 16 / G, i_last = min(rb * 16 + 15, rows - 1) / G;
+    for (int rb = 0; rb * BLOCK < rows; ++rb) {
+        const int row_a = rb * BLOCK + gid, row_b = row_a + 8;     // (row_b with HI only)
+        const int i_first = rb * BLOCK / G, i_last = min(rb * BLOCK + BLOCK - 1, rows - 1) / G;
         // rows behind the last one copy its position: never stored
         const int pos_a = len - n_q + min(row_a, rows - 1) / G;
         const int pos_b = len - n_q + min(row_b, rows - 1) / G;
@@ -327,7 +327,7 @@ __global__ void __launch_bounds__(WARPS * 32) row_attn_kernel(const RowAttnParam
                 *reinterpret_cast<float2*>(&wacc[(gid + 8) * RACC_PITCH + 8 * nt + 2 * tig]) =
                     make_float2(acc[nt][2], acc[nt][3]);
         }
-        const int nr = min(16, rows - rb * 16), n_el = nr * (PR_HD / 4);
+        const int nr = min(BLOCK, rows - rb * BLOCK), n_el = nr * (PR_HD / 4);
         if (CLUSTER) cg::this_cluster().sync(); // peers run, and are done with xacc
         else __syncthreads();
         // four channels of a row: (m, l, O) over the CTA's warps
@@ -348,7 +348,7 @@ __global__ void __launch_bounds__(WARPS * 32) row_attn_kernel(const RowAttnParam
             return o;
         };
         auto finish = [&](int row, int d, float M, float L, float4 o) {
-            const int at = rb * 16 + row, i = at / G, h = kh * G + at - i * G;
+            const int at = rb * BLOCK + row, i = at / G, h = kh * G + at - i * G;
             if (p.parts_o) {
                 // one of several parts
                 const int64_t x = (p.part + (CLUSTER ? 0 : c)) * p.part_rows +
@@ -373,7 +373,7 @@ __global__ void __launch_bounds__(WARPS * 32) row_attn_kernel(const RowAttnParam
                 const float4 o = warps_sum(row, d, M, L);
                 finish(row, d, M, L, o);
             }
-            if ((rb + 1) * 16 < rows) __syncthreads();          // the rings are idle again
+            if ((rb + 1) * BLOCK < rows) __syncthreads();       // the rings are idle again
         } else {
             // CTA k finishes the four-channel pieces [k per, (k + 1) per)
             cg::cluster_group cluster = cg::this_cluster();

@@ -200,11 +200,10 @@ struct FindState {
     int s0, before;
 };
 
-// Work item `w` of `total` tiles x KV heads x parts, tiles fastest, by one warp; false:
-// there is no such tile (total an upper bound).
-__device__ __forceinline__ bool find_item(const TileAttnParams& p, int w, int total, int lane,
-                                          FindState& at, Item& it) {
-    const int target = w % total, rest = w / total;
+// Row tile `target` with KV head and part `rest`, by one warp; false: there is no such
+// tile (the tiles were not counted).
+__device__ __forceinline__ bool find_item(const TileAttnParams& p, int target, int rest,
+                                          int lane, FindState& at, Item& it) {
     if (target < at.before) at = {0, 0};
     for (; at.s0 < p.n_seg; at.s0 += 32) {
         const int s0 = at.s0, before = at.before;
@@ -322,14 +321,21 @@ tile_attn_kernel(const __grid_constant__ CUtensorMap map_q,
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
         if (warp == 10) {
             // ---- items ----------------------------------------------------------------
+            // (tiles fastest; those nobody expects come behind all the others)
             const int tiles = p.tile_bound ? p.tile_bound : count_tiles(p, lane);
-            const int total = tiles * p.r.n_kv * p.parts;
+            const int expected = tiles * p.r.n_kv * p.parts;
+            const int total = expected + p.tile_more * p.r.n_kv * p.parts;
             FindState at = {0, 0};
             int n = 0;
             for (int w = blockIdx.x; !__any_sync(0xffffffffu, is_dead(sm)); w += gridDim.x) {
                 Item it;
                 it.valid = 0;
-                if (w < total && !find_item(p, w, tiles, lane, at, it)) continue;
+                if (w < total) {
+                    const int n_tiles = w < expected ? tiles : p.tile_more;
+                    const int x = w < expected ? w : w - expected, rest = x / n_tiles;
+                    const int target = x - rest * n_tiles + (w < expected ? 0 : tiles);
+                    if (!find_item(p, target, rest, lane, at, it)) continue;
+                }
                 if (n >= 2)
                     ta_wait(sm, &sm.item_empty[n & 1], (uint32_t)((n >> 1) - 1) & 1u, p.status);
                 if (lane == 0) {
@@ -921,7 +927,7 @@ __global__ void __launch_bounds__(32 * TJ_WARPS) join_parts_kernel(const TileAtt
 
 }  // namespace
 
-int launch_tile_attn(const char* who, TileAttnParams p, int max_tiles, int n_tok,
+int launch_tile_attn(const char* who, TileAttnParams p, int tiles, int max_tiles, int n_tok,
                      cudaStream_t s) {
     p.head_chunks = p.r.n_kv > 1 ? (int)(p.r.sh / 64) : 0;
     CUtensorMap mq = {}, mk, mv;
@@ -942,10 +948,13 @@ int launch_tile_attn(const char* who, TileAttnParams p, int max_tiles, int n_tok
                              smem);
         attr_done[dev] = true;
     }
-    const int64_t items = (int64_t)max_tiles * p.r.n_kv * p.parts;
-    LOCKS_REQUIRE(items < (1 << 30), LOCKS_ERR_SIZE, "%s: too many query rows in one call", who);
-    // (with a CTA for every tile there could be, nobody has to count them first)
-    p.tile_bound = items <= sm_count() ? max_tiles : 0;
+    const int64_t items = (int64_t)tiles * p.r.n_kv * p.parts;
+    LOCKS_REQUIRE((int64_t)max_tiles * p.r.n_kv * p.parts < (1 << 30), LOCKS_ERR_SIZE,
+                  "%s: too many query rows in one call", who);
+    // (with a CTA for every tile that is expected, nobody has to count them first: what
+    // there is beyond is looked for while those are computed)
+    p.tile_bound = items <= sm_count() ? tiles : 0;
+    p.tile_more = p.tile_bound ? max_tiles - tiles : 0;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(items < sm_count() ? items : sm_count()), 1, 1);
     cfg.blockDim = dim3(TA_THREADS, 1, 1);

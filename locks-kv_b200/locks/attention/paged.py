@@ -60,8 +60,9 @@ def window_paged_attention(q: torch.Tensor, kv_cache: torch.Tensor,
     position p sees keys j <= p with p - j < ``window`` or j < ``sinks``
     (``window`` None: all of them).  Rows that see nothing become 0 (lse -inf),
     rows behind ``cu_q[R]`` stay as they were, pages that nobody sees are not read.
-    ``max_q`` bounds the query tokens of a request (rows of one with more may be
-    left out).  ``scratch``: fp32 workspace that lets the long keys of few queries be
+    ``max_q``: the query tokens of the longest request; it steers how the work is cut,
+    a request with more is answered all the same, more slowly (0: nothing is done).
+    ``scratch``: fp32 workspace that lets the long keys of few queries be
     cut into parts, see :func:`attention_scratch_floats`; calls that may overlap on
     the GPU need one each.  ``status``: int32, set where a bounded wait ran out."""
     dev = _cabi.one_device(q, kv_cache, block_table, cu_q, seq_lens, out, scratch, lse,

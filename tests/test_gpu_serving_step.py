@@ -292,6 +292,41 @@ def test_window_short_table_and_small_bound():
                                          2 ** 31 - 1, 0))
 
 
+BEYOND_BOUND_CASES = [
+    # (n_kv, G, [(new, cached)], max_q): requests with more query tokens than max_q says
+    (2, 4, [(5, 200)], 1),                                  # few pairs, eight-row blocks
+    (2, 4, [(41, 300), (1, 20), (2, 90)], 2),
+    (1, 12, [(50, 90), (1, 64)], 1),                        # sixteen-row blocks
+    (2, 4, [(3, 60 + r) for r in range(45)] + [(30, 100)], 2),      # many pairs
+    (1, 8, [(3, 34000), (1, 33000)], 1),                    # few rows, very long
+    (2, 8, [(300, 310), (1, 40), (700, 2000), (2, 2)], 20),         # tiles, in parts with scratch
+    (8, 4, [(33, 100)] * 40 + [(400, 900)], 6),
+]
+
+
+@pytest.mark.parametrize("case", range(len(BEYOND_BOUND_CASES)))
+def test_window_requests_with_more_queries_than_the_bound(case):
+    """The bound steers how the work is cut, not what is computed: a call captured for
+    fewer tokens meets longer requests."""
+    n_kv, G, reqs, max_q = BEYOND_BOUND_CASES[case]
+    lens = [l for _, l in reqs]
+    g, cache, k, v, table = paged(70 + case, lens, n_kv)
+    cu = [0]
+    for n, _ in reqs:
+        cu.append(cu[-1] + n)
+    T, H = cu[-1], n_kv * G
+    q = torch.randn(T + 2, H, 128, device=DEV, generator=g).to(BF16)
+    for scratch in (None, torch.full((2 ** 23,), float("nan"), device=DEV)):
+        out = torch.full((T + 2, H, 128), 7.0, device=DEV, dtype=BF16)
+        lse = torch.full((T + 2, H), 7.0, device=DEV)
+        run_window(q, cache, table, i32(cu), i32(lens), n_kv, G, None, 0, max_q, out=out, lse=lse,
+                   scratch=scratch)
+        assert bool((out[T:] == 7).all()) and bool((lse[T:] == 7).all())
+        for r, (n, l) in enumerate(reqs):
+            at = slice(cu[r], cu[r + 1])
+            check(out[at], lse[at], want_window(q[at], k, v, table[r], l, n, 2 ** 31 - 1, 0), r)
+
+
 def test_window_many_requests_few_of_them_long():
     """Several hundred requests, most with one token, prompts between them."""
     n_kv, G, R = 1, 8, 700
