@@ -624,6 +624,8 @@ int locks_dense_decode(const void* q, int64_t q_stride_req, const void* k_cache,
  * nothing becomes 0 with lse -inf; tokens behind cu_q[n_req] are left as they were.
  * Pages that no query of a request sees are not read: their table entries may hold
  * anything.  Keys and values of the seen pages must be finite up to seq_lens[r].
+ * A query row need not be: one with a seen score of NaN or +inf becomes NaN, its lse
+ * too (a score of -inf has weight 0), and no other row is affected.
  * Block ids are clamped to [0, num_blocks), keys end with the table's last column,
  * query runs with the last row of q (n_tok).  scale must be positive.
  * lse: optional f32 natural log-sum-exp, lse[token * lse_stride_tok + head].

@@ -63,7 +63,8 @@ __device__ __forceinline__ PageList page_list(int pos_lo, int pos_hi, int window
 }
 
 // Row `at` of several partial results: channels d .. d + 3 of O, with the maximum (in
-// log2 units) and the sum.  A part that saw nothing carries l = 0 and no O.
+// log2 units) and the sum.  A part that saw nothing carries l = 0 and no O; a sum of NaN
+// makes the row NaN.
 struct PartSum {
     float m, l;
     float4 o;
@@ -85,15 +86,15 @@ __device__ __forceinline__ PartSum join_parts(const float* o, const float* ml, i
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
             if (s0 + k >= parts) x[k].y = 0.f;
-            if (x[k].y > 0.f) up = fmaxf(up, x[k].x);
+            if (x[k].y != 0.f) up = fmaxf(up, x[k].x);
         }
-        const float a = r.l > 0.f ? pr_exp2(r.m - up) : 0.f;
+        const float a = r.l != 0.f ? pr_exp2(r.m - up) : 0.f;
         r.l *= a;
         r.o.x *= a; r.o.y *= a; r.o.z *= a; r.o.w *= a;
         r.m = up;
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-            if (x[k].y > 0.f) {                 // (a part without keys wrote no O)
+            if (x[k].y != 0.f) {                // (a part without keys wrote no O)
                 const float w = pr_exp2(x[k].x - up);
                 r.l += w * x[k].y;
                 r.o.x += w * v[k].x; r.o.y += w * v[k].y;

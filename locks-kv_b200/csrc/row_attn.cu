@@ -340,7 +340,7 @@ __global__ void __launch_bounds__(WARPS * 32) row_attn_kernel(const RowAttnParam
 #pragma unroll
             for (int w = 0; w < WARPS; ++w) {
                 const float lw = sm.cl[w][row];
-                const float wt = lw > 0.f ? pr_exp2(sm.cm[w][row] - M) : 0.f;
+                const float wt = lw != 0.f ? pr_exp2(sm.cm[w][row] - M) : 0.f;
                 L += wt * lw;
                 axpy4(o, wt, *reinterpret_cast<const float4*>(
                                  reinterpret_cast<const float*>(&sm.wb[w]) + row * RACC_PITCH + d));
@@ -358,13 +358,14 @@ __global__ void __launch_bounds__(WARPS * 32) row_attn_kernel(const RowAttnParam
                     *reinterpret_cast<float2*>(p.parts_ml + 2 * x) = make_float2(M, L);
                 return;
             }
-            const float inv = L > 0.f ? 1.f / L : 0.f;
+            // (a sum that is NaN makes the row NaN: only 0 is a row that saw nothing)
+            const float inv = L != 0.f ? 1.f / L : 0.f;
             *reinterpret_cast<uint2*>(p.out + (int64_t)(tok0 + i) * p.o_tok +
                                       (int64_t)h * p.o_head + d) =
                 make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
             if (d == 0 && p.lse)
                 p.lse[(int64_t)(tok0 + i) * p.lse_tok + h] =
-                    L > 0.f ? (M + log2f(L)) * PR_LN2 : -INFINITY;
+                    L != 0.f ? (M + log2f(L)) * PR_LN2 : -INFINITY;
         };
         if (!CLUSTER) {
             for (int e = tid; e < n_el; e += THREADS) {
@@ -399,7 +400,7 @@ __global__ void __launch_bounds__(WARPS * 32) row_attn_kernel(const RowAttnParam
 #pragma unroll 4
                 for (int k = 0; k < CL; ++k) {
                     const float lk = sm.xl[k][row];
-                    const float wt = lk > 0.f ? pr_exp2(sm.xm[k][row] - M) : 0.f;
+                    const float wt = lk != 0.f ? pr_exp2(sm.xm[k][row] - M) : 0.f;
                     L += wt * lk;
                     axpy4(o, wt, *reinterpret_cast<const float4*>(
                                      &sm.xacc[4 * (k * per + e - c * per)]));

@@ -79,9 +79,15 @@ struct __align__(1024) TileSmem {
 static_assert(sizeof(TileSmem) + 1024 <= 232448, "one CTA's shared memory");
 constexpr int TA_READERS = 11;                     // warps that read an item: all but its finder
 
+// maxima that a NaN goes through
+__device__ __forceinline__ float max2(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
 // two fp32 operations in one instruction
@@ -642,7 +648,7 @@ tile_attn_kernel(const __grid_constant__ CUtensorMap map_q,
                     for (int c = c0; c < c0 + 64; c += 16)
 #pragma unroll
                         for (int e = 0; e < 8; ++e)
-                            mx[e] = c == 0 ? fmaxf(s[e], s[8 + e]) : max3(mx[e], s[c + e], s[c + 8 + e]);
+                            mx[e] = c == 0 ? max2(s[e], s[8 + e]) : max3(mx[e], s[c + e], s[c + 8 + e]);
                 };
                 tc_ld32(ts, sr);
                 tc_ld32(ts + 32, sr + 32);
@@ -683,7 +689,7 @@ tile_attn_kernel(const __grid_constant__ CUtensorMap map_q,
                     peaks(64);
                 }
                 const float tile_max = max3(max3(mx[0], mx[1], mx[2]), max3(mx[3], mx[4], mx[5]),
-                                            fmaxf(mx[6], mx[7]));
+                                            max2(mx[6], mx[7]));
                 if (t == 0) {
                     m = tile_max;
                 } else if (__any_sync(0xffffffffu, (tile_max - m) * sl2 > TA_RAISE)) {
@@ -707,7 +713,12 @@ tile_attn_kernel(const __grid_constant__ CUtensorMap map_q,
                         tc_st16(to + 16 * c, o);
                     }
                 }
-                const float base = m == -INFINITY ? 0.f : m * sl2;
+                // A score of NaN or +inf makes the row NaN: its maximum becomes NaN, with
+                // it every exponent, and so l and O (three of four exponentials are the
+                // special-function unit's; the polynomial turns NaN into 0)
+                if (tile_max != tile_max) m = tile_max;
+                const float ml2 = m * sl2;
+                const float base = m == -INFINITY ? 0.f : fmaf(ml2, 0.f, ml2);
                 const float2 k2 = make_float2(sl2, sl2), b2 = make_float2(-base, -base);
                 float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
@@ -742,7 +753,8 @@ tile_attn_kernel(const __grid_constant__ CUtensorMap map_q,
             }
             // streams that share the rows: each finishes half of the channels
             const int chunk0 = by_rows ? 0 : 2 * i, chunks = by_rows ? 4 : 2;
-            float w_mine = l > 0.f ? 1.f : 0.f, w_other = 0.f;
+            // (a sum that is NaN is not zero: the row is NaN, not one that saw nothing)
+            float w_mine = l != 0.f ? 1.f : 0.f, w_other = 0.f;
             if (!by_rows) {
                 float2* mine = reinterpret_cast<float2*>(sm.stage[warp]) + lane;
                 *mine = make_float2(m, l);
@@ -753,13 +765,13 @@ tile_attn_kernel(const __grid_constant__ CUtensorMap map_q,
                 meet();
                 const float m1 = other.x, l1 = other.y;
                 const float up = fmaxf(m, m1);
-                w_mine = l > 0.f ? pr_exp2((m - up) * sl2) : 0.f;
-                w_other = l1 > 0.f ? pr_exp2((m1 - up) * sl2) : 0.f;
+                w_mine = l != 0.f ? pr_exp2((m - up) * sl2) : 0.f;
+                w_other = l1 != 0.f ? pr_exp2((m1 - up) * sl2) : 0.f;
                 l = w_mine * l + w_other * l1;
                 m = up;
             }
             const bool final = p.parts_out == nullptr;
-            const float inv = !final ? 1.f : l > 0.f ? 1.f / l : 0.f;
+            const float inv = !final ? 1.f : l != 0.f ? 1.f / l : 0.f;
             w_mine *= inv;
             w_other *= inv;
             const int64_t part_at = (int64_t)part * p.part_rows +
@@ -771,7 +783,7 @@ tile_attn_kernel(const __grid_constant__ CUtensorMap map_q,
                                          : part_at * (PR_HD * 4);
             uint8_t* dst = final ? reinterpret_cast<uint8_t*>(p.r.out)
                                  : reinterpret_cast<uint8_t*>(p.parts_out);
-            const bool any = __any_sync(0xffffffffu, l > 0.f);
+            const bool any = __any_sync(0xffffffffu, l != 0.f);
             uint8_t* stage = sm.stage[warp];
             const int live = min(n_rows - (by_rows ? i * TA_TILE : 0) - q4 * 32, 32);
             int64_t off[8];
@@ -811,8 +823,8 @@ tile_attn_kernel(const __grid_constant__ CUtensorMap map_q,
                 const float w2 = by_rows ? w_mine : w_other;
 #pragma unroll
                 for (int e = 0; e < 64; ++e) {
-                    f[e] = w_mine > 0.f ? w_mine * f[e] : 0.f;
-                    f[64 + e] = w2 > 0.f ? w2 * f[64 + e] : 0.f;
+                    f[e] = w_mine != 0.f ? w_mine * f[e] : 0.f;
+                    f[64 + e] = w2 != 0.f ? w2 * f[64 + e] : 0.f;
                 }
                 if (!by_rows)
 #pragma unroll
@@ -842,10 +854,10 @@ tile_attn_kernel(const __grid_constant__ CUtensorMap map_q,
             if (local < n_rows && (by_rows || i == 0)) {
                 if (!final)         // O is relative to m; (m in log2 units, l)
                     *reinterpret_cast<float2*>(p.parts_ml + 2 * part_at) =
-                        make_float2(l > 0.f ? m * sl2 : -INFINITY, l);
+                        make_float2(l != 0.f ? m * sl2 : -INFINITY, l);
                 else if (p.r.lse)
                     p.r.lse[(int64_t)(t0 + tok) * p.r.lse_tok + head] =
-                        l > 0.f ? (m * sl2 + log2f(l)) * PR_LN2 : -INFINITY;
+                        l != 0.f ? (m * sl2 + log2f(l)) * PR_LN2 : -INFINITY;
             }
             tc_before_sync();
             // (the other stream has read this one's O and sums before they change)
@@ -916,13 +928,13 @@ __global__ void __launch_bounds__(32 * TJ_WARPS) join_parts_kernel(const TileAtt
         if (n == 0) return;                         // the few-row kernel's
     }
     const PartSum s = join_parts(p.parts_out, p.parts_ml, p.part_rows, parts, at, 4 * lane);
-    const float inv = s.l > 0.f ? 1.f / s.l : 0.f;
+    const float inv = s.l != 0.f ? 1.f / s.l : 0.f;
     *reinterpret_cast<uint2*>(p.r.out + (int64_t)tok * p.r.o_tok + (int64_t)h * p.r.o_head +
                               4 * lane) =
         make_uint2(pack_bf16x2(s.o.x * inv, s.o.y * inv), pack_bf16x2(s.o.z * inv, s.o.w * inv));
     if (lane == 0 && p.r.lse)
         p.r.lse[(int64_t)tok * p.r.lse_tok + h] =
-            s.l > 0.f ? (s.m + log2f(s.l)) * PR_LN2 : -INFINITY;
+            s.l != 0.f ? (s.m + log2f(s.l)) * PR_LN2 : -INFINITY;
 }
 
 }  // namespace

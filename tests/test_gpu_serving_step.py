@@ -425,6 +425,69 @@ def test_empty_batches():
     assert got["slots"] == [-1] * 3 and got["taken"] == 1 and got["cu"] == [0]
 
 
+NOT_FINITE_CASES = [
+    # (n_kv, G, [(new, cached)], window, sinks): one for each way through the kernels
+    (2, 4, [(1, 300), (2, 40)], None, 0),                       # few rows, clusters
+    (1, 12, [(3, 77)], 20, 3),
+    (2, 4, [(1, 90 + r) for r in range(60)], None, 0),          # many pairs
+    (1, 8, [(1, 34000)], None, 0),                              # cut into parts with scratch
+    (2, 4, [(30, 200), (100, 700)], None, 0),                   # tiles of shared and of own rows
+    (2, 3, [(80, 300), (1, 9)], 64, 5),
+    (1, 8, [(40, 9000)], None, 0),                              # tiles, parts with scratch
+    (1, 4, [(120, 120)], 1, 0),                                 # one key to a row, every column
+    (1, 4, [(20, 60)], 0, 0),                                   # no key: nothing to be wrong
+]
+
+
+def spoil(q, g):
+    """NaN and infinities in single channels of scattered rows."""
+    T, H, _ = q.shape
+    at = torch.randperm(T * H, device=DEV, generator=g)[:max(3, T * H // 7)]
+    for i, bad in enumerate((float("nan"), float("inf"), -float("inf"))):
+        rows = at[i::3]
+        q[rows // H, rows % H, (rows * 13 + 5 * i) % 128] = bad
+
+
+def check_not_finite(q, out, lse, k, v, seen, r=""):
+    """A seen score of NaN or +inf makes its row NaN; the other rows are what they are."""
+    G = q.shape[1] // k.shape[1]
+    x = torch.einsum("nhd,jhd->nhj", q.double(), k.double().repeat_interleave(G, 1)) * SCALE
+    lost = ((x.isnan() | (x == math.inf)) & seen[:, None]).any(-1)
+    assert bool(out[lost].isnan().all()) and bool(lse[lost].isnan().all()), r
+    clean = q.isfinite().all(-1)
+    some = seen.any(-1)
+    assert bool((lost | clean | ~some[:, None] | (x.masked_fill(~seen[:, None], -math.inf) ==
+                                                  -math.inf).all(-1)).all())
+    none = ~lost & ~clean
+    assert bool((out[none] == 0).all()) and bool((lse[none] == -math.inf).all()), r
+    want = ref.attend(torch.where(clean[..., None], q, 0), k, v, seen, SCALE)
+    check(out[clean], lse[clean], [t[clean] for t in want], r)
+
+
+@pytest.mark.parametrize("case", range(len(NOT_FINITE_CASES)))
+def test_window_queries_that_are_not_finite(case):
+    n_kv, G, reqs, window, sinks = NOT_FINITE_CASES[case]
+    lens = [l for _, l in reqs]
+    g, cache, k, v, table = paged(90 + case, lens, n_kv)
+    w = 2 ** 31 - 1 if window is None else window
+    cu = [0]
+    for n, _ in reqs:
+        cu.append(cu[-1] + n)
+    q = torch.randn(cu[-1], n_kv * G, 128, device=DEV, generator=g).to(BF16)
+    spoil(q, g)
+    for scratch in (None, torch.empty(2 ** 23, device=DEV)):
+        lse = torch.full(q.shape[:2], 7.0, device=DEV)
+        out = torch.full_like(q, 7.0)
+        run_window(q, cache, table, i32(cu), i32(lens), n_kv, G, window, sinks,
+                   max(n for n, _ in reqs), out=out, lse=lse, scratch=scratch)
+        for r, (n, l) in enumerate(reqs):
+            at = slice(cu[r], cu[r + 1])
+            pos, key = torch.arange(l - n, l, device=DEV)[:, None], torch.arange(l, device=DEV)[None]
+            seen = (key <= pos) & ((pos - key < w) | (key < sinks))
+            check_not_finite(q[at], out[at], lse[at], ref.gather(k, table[r], l),
+                             ref.gather(v, table[r], l), seen, r)
+
+
 def test_bounds_beyond_the_queries_are_cut_off():
     """cu_q that runs past q (fewer rows than it says): the rows that exist are right,
     nothing behind them is touched."""
@@ -581,6 +644,26 @@ def test_prefix(case, more):
     for r, l in enumerate(lens):
         want = want_window(q[r:r + 1], cache[:, 0], cache[:, 1], table[r], l, 1, 2 ** 31 - 1, 0)
         check(out[r:r + 1], lse[r:r + 1], want, r)
+
+
+@pytest.mark.parametrize("case", [3, 5, 7, 9, 10])
+def test_prefix_queries_that_are_not_finite(case):
+    n_kv, G, groups = PREFIX_CASES[case]
+    g, cache, table, lens = prefix_paged(case, groups, n_kv)
+    R, H = len(lens), n_kv * G
+    cu = [0]
+    for _, ls in groups:
+        cu.append(cu[-1] + len(ls))
+    q = torch.randn(R, H, 128, device=DEV, generator=g).to(BF16)
+    spoil(q, g)
+    for more in (2, 64):
+        lse = torch.full((R, H), 7.0, device=DEV)
+        out = run_prefix(q, cache, table, lens, cu, [p for p, _ in groups], n_kv, G, lse=lse,
+                         floats=more * R * H * 130)
+        for r, l in enumerate(max(x, 0) for x in lens):
+            check_not_finite(q[r:r + 1], out[r:r + 1], lse[r:r + 1], ref.gather(cache[:, 0], table[r], l),
+                             ref.gather(cache[:, 1], table[r], l),
+                             torch.ones(1, l, dtype=torch.bool, device=DEV), r)
 
 
 def test_prefix_rows_outside_groups_and_empty_groups():
