@@ -362,8 +362,10 @@ tile_attn_kernel(const __grid_constant__ CUtensorMap map_q,
                           kh = item->kh, n_tiles = item->n_tiles;
                 done_with(n);
                 if (n_tiles == 0) continue;
-                if (loads > 0)
+                if (loads > 0) {
                     ta_wait(sm, &sm.q_empty, (uint32_t)(loads - 1) & 1u, p.status);
+                    if (__any_sync(0xffffffffu, is_dead(sm))) break;    // Q is in use still
+                }
                 ++loads;
                 const int subs = n_rows > TA_TILE ? 2 : 1;
                 both += subs - 1;
@@ -475,9 +477,12 @@ tile_attn_kernel(const __grid_constant__ CUtensorMap map_q,
                 }
             }
             // a wait ran out: nobody consumed the last copies; they must land all the same
+            // (those of a tile with a cut page complete on `tail`, and only the last such
+            // tile's can be under way)
             if (__any_sync(0xffffffffu, is_dead(sm)))
-                for (int i = max(issued - TA_RING, 0); i < issued; ++i)
-                    mbar_wait(&sm.full[i % TA_RING], (uint32_t)(i / TA_RING) & 1u, p.status);
+                for (int i = max(issued - TA_RING, 0); i < issued + min(cuts, 1); ++i)
+                    mbar_wait(i < issued ? &sm.full[i % TA_RING] : &sm.tail,
+                              (uint32_t)(i < issued ? i / TA_RING : cuts - 1) & 1u, p.status);
         } else if (warp == 8) {
             // ---- products -------------------------------------------------------------
             constexpr uint32_t ID_S = tc_idesc(TA_TILE, false), ID_O = tc_idesc(PR_HD, true);

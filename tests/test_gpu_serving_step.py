@@ -327,6 +327,27 @@ def test_window_requests_with_more_queries_than_the_bound(case):
             check(out[at], lse[at], want_window(q[at], k, v, table[r], l, n, 2 ** 31 - 1, 0), r)
 
 
+@pytest.mark.parametrize("G", [4, 3])
+def test_window_tiles_that_end_at_every_offset_of_a_page(G):
+    """More tiles than SMs, so that a CTA takes several in a row, each with a last page
+    that is cut off at another token; what lies behind is not finite."""
+    n_kv, n = 4, 34
+    lens = [200 + 17 * r for r in range(96)]
+    g, cache, k, v, table = paged(60 + G, lens, n_kv)
+    for r, l in enumerate(lens):
+        if l % 16:
+            k[table[r, l // 16], l % 16:] = float("nan")
+            v[table[r, l // 16], l % 16:] = float("inf")
+    q = torch.randn(n * len(lens), n_kv * G, 128, device=DEV, generator=g).to(BF16)
+    cu = i32([n * r for r in range(len(lens) + 1)])
+    lse = torch.full(q.shape[:2], 7.0, device=DEV)
+    out = run_window(q, cache, table, cu, i32(lens), n_kv, G, 150, 5, n, lse=lse)
+    kk, vv = k.nan_to_num(0, 0, 0), v.nan_to_num(0, 0, 0)
+    for r, l in enumerate(lens):
+        at = slice(n * r, n * r + n)
+        check(out[at], lse[at], want_window(q[at], kk, vv, table[r], l, n, 150, 5), r)
+
+
 def test_window_many_requests_few_of_them_long():
     """Several hundred requests, most with one token, prompts between them."""
     n_kv, G, R = 1, 8, 700
