@@ -14,7 +14,7 @@ import torch
 from .. import _cabi
 from .decode import _planes
 
-NO_WINDOW = 2 ** 31 - 1
+NO_WINDOW = 2 ** 31 - 1      # larger counts than the entry point's integers hold mean all
 
 
 def _checked(q, kv_cache, block_table, out, lse, scratch, n_kv, G, ints):
@@ -74,9 +74,9 @@ def window_paged_attention(q: torch.Tensor, kv_cache: torch.Tensor,
     if R == 0 or q.shape[0] == 0:
         return
     _cabi.call_on(dev, "locks_window_attention", *source, cu_q.data_ptr(),
-                  seq_lens.data_ptr(), *target, q.shape[0], R, max_q, n_kv, G, d, page,
-                  NO_WINDOW if window is None else min(window, NO_WINDOW), sinks,
-                  scale, _cabi.addr(status))
+                  seq_lens.data_ptr(), *target, q.shape[0], R, min(max_q, NO_WINDOW), n_kv,
+                  G, d, page, NO_WINDOW if window is None else min(window, NO_WINDOW),
+                  min(sinks, NO_WINDOW), scale, _cabi.addr(status))
 
 
 def shared_prefix_paged_decode(q: torch.Tensor, kv_cache: torch.Tensor,

@@ -348,6 +348,19 @@ def test_window_tiles_that_end_at_every_offset_of_a_page(G):
         check(out[at], lse[at], want_window(q[at], kk, vv, table[r], l, n, 150, 5), r)
 
 
+@pytest.mark.parametrize("n,G", [(1, 4), (60, 8)])
+def test_window_counts_beyond_32_bits(n, G):
+    """More first tokens, a wider window or a larger bound than 32 bits hold: all of them."""
+    g, cache, k, v, table = paged(33, [300], 2)
+    q = torch.randn(n, 2 * G, 128, device=DEV, generator=g).to(BF16)
+    want = run_window(q, cache, table, i32([0, n]), i32([300]), 2, G, None, 0, n)
+    for window, sinks, max_q in ((10, 2 ** 32, n), (2 ** 33, 0, n), (None, 0, 2 ** 32)):
+        got = run_window(q, cache, table, i32([0, n]), i32([300]), 2, G, window, sinks, max_q)
+        # (another bound may cut the work another way)
+        check(got, None, want_window(q, k, v, table[0], 300, n, 2 ** 31 - 1, 0))
+        assert max_q != n or torch.equal(got, want)
+
+
 def test_window_many_requests_few_of_them_long():
     """Several hundred requests, most with one token, prompts between them."""
     n_kv, G, R = 1, 8, 700
