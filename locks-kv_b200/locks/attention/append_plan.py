@@ -38,6 +38,7 @@ def append_plan(seq_lens: torch.Tensor, n_new: torch.Tensor,
             "lengths, counts and the free list are contiguous int32"
     assert slot_mapping.dtype is i64 and slot_mapping.is_contiguous()
     assert positions.dtype is i64 and positions.is_contiguous()
+    assert status is None or status.dtype is i32, "status is int32"
     R, cap = seq_lens.numel(), slot_mapping.numel()
     rows, width = block_table.shape
     stride = block_table.stride()

@@ -17,7 +17,7 @@ from .decode import _planes
 NO_WINDOW = 2 ** 31 - 1      # larger counts than the entry point's integers hold mean all
 
 
-def _checked(q, kv_cache, block_table, out, lse, scratch, n_kv, G, ints):
+def _checked(q, kv_cache, block_table, out, lse, scratch, status, n_kv, G, ints):
     """What both calls check of their tensors; the arguments both pass on."""
     k, v, (n_blocks, page, heads, d), cs = _planes(kv_cache)
     bf16, f32, i32 = torch.bfloat16, torch.float32, torch.int32
@@ -31,6 +31,7 @@ def _checked(q, kv_cache, block_table, out, lse, scratch, n_kv, G, ints):
     for t in ints:
         assert t.dtype is i32 and t.is_contiguous(), \
             "lengths and bounds are contiguous int32"
+    assert status is None or status.dtype is i32, "status is int32"
     lse_at, lse_stride, scratch_at, floats = None, 0, None, 0
     if lse is not None:
         lse_stride, one = lse.stride()
@@ -68,7 +69,7 @@ def window_paged_attention(q: torch.Tensor, kv_cache: torch.Tensor,
     dev = _cabi.one_device(q, kv_cache, block_table, cu_q, seq_lens, out, scratch, lse,
                            status)
     source, target, d, page = _checked(q, kv_cache, block_table, out, lse, scratch,
-                                       n_kv, G, (cu_q, seq_lens))
+                                       status, n_kv, G, (cu_q, seq_lens))
     R = seq_lens.numel()
     assert cu_q.numel() == R + 1 and block_table.shape[0] == R
     if R == 0 or q.shape[0] == 0:
@@ -95,7 +96,7 @@ def shared_prefix_paged_decode(q: torch.Tensor, kv_cache: torch.Tensor,
     dev = _cabi.one_device(q, kv_cache, block_table, seq_lens, cu_groups, prefix_lens,
                            out, scratch, lse, status)
     source, target, d, page = _checked(q, kv_cache, block_table, out, lse, scratch,
-                                       n_kv, G, (seq_lens, cu_groups, prefix_lens))
+                                       status, n_kv, G, (seq_lens, cu_groups, prefix_lens))
     R, groups = q.shape[0], prefix_lens.numel()
     assert seq_lens.numel() == block_table.shape[0] == R
     assert cu_groups.numel() == groups + 1

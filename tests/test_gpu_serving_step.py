@@ -361,6 +361,27 @@ def test_window_counts_beyond_32_bits(n, G):
         assert max_q != n or torch.equal(got, want)
 
 
+def test_status_of_another_type_is_refused():
+    from locks.attention import (append_plan, attention_scratch_floats, shared_prefix_paged_decode,
+                                 window_paged_attention)
+    g, cache, k, v, table = paged(34, [40], 2)
+    q = torch.randn(1, 8, 128, device=DEV, generator=g).to(BF16)
+    lens, cu = i32([40]), i32([0, 1])
+    wide = torch.zeros(1, dtype=I64, device=DEV)
+    for st in (wide.clone(), torch.zeros(1, dtype=torch.bool, device=DEV)):
+        with pytest.raises(AssertionError, match="status"):
+            window_paged_attention(q, cache, table, cu, lens, torch.empty_like(q), n_kv=2, G=4,
+                                   window=None, scale=SCALE, max_q=1, status=st)
+        with pytest.raises(AssertionError, match="status"):
+            shared_prefix_paged_decode(q, cache, table, lens, cu, i32([16]), torch.empty_like(q), n_kv=2,
+                                       G=4, scale=SCALE, status=st,
+                                       scratch=torch.empty(attention_scratch_floats(1, 8), device=DEV))
+        with pytest.raises(AssertionError, match="status"):
+            append_plan(lens, i32([1]), table, i32([1]), i32([0]), slot_mapping=wide, positions=wide.clone(),
+                        cu_tokens=cu, lens_out=lens, taken_out=i32([0]), status=st)
+        assert int(st) == 0
+
+
 def test_window_many_requests_few_of_them_long():
     """Several hundred requests, most with one token, prompts between them."""
     n_kv, G, R = 1, 8, 700
