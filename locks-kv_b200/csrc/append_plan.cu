@@ -197,9 +197,13 @@ extern "C" int locks_append_plan(const int32_t* seq_lens, const int32_t* n_new,
     p.slot = slot_mapping; p.pos = positions; p.cu = cu_tokens;
     p.lens_out = lens_out; p.taken_out = taken_out;
     p.status = status; p.n_req = n_req; p.cap = max_tokens; p.page = page;
-    // 16 requests, one token each: 3.7 us with 128 threads, 5.5 with 1024; 256 requests,
-    // 65536 tokens: 11 us with 16 CTAs of 1024, 20 with 8 of 512
-    const bool few = n_req <= 2 * AP_FEW && max_tokens <= 4 * AP_FEW;
+    // One small CTA while a thread has about two requests and two tokens at most.  Calls
+    // in a graph, us, 128 threads against CTAs of 1024 (a wider scan, but a barrier of 32
+    // warps), requests x tokens of the step: 1 x 1 2.9 and 4.7, 16 x 128 3.1 and 4.9,
+    // 64 x 256 4.1 and 5.0, 256 x 256 4.8 and 5.2; on the other side 16 x 512 5.1 and 4.9,
+    // 64 x 512 5.9 and 5.1, 256 x 512 7.0 and 5.4, 512 x 512 7.9 and 5.6, 1024 x 1024 14.7
+    // and 6.7.  256 requests, 65536 tokens: 11 with 16 CTAs of 1024, 20 with 8 of 512.
+    const bool few = n_req <= 2 * AP_FEW && max_tokens <= 2 * AP_FEW;
     void (*kernel)(const PlanParams) =
         few ? append_plan_kernel<AP_FEW> : append_plan_kernel<AP_MANY>;
     const int smem = (3 * n_req + 1) * (int)sizeof(int);
