@@ -27,8 +27,9 @@
 //
 // P is split into two bf16 terms (P = hi + lo to 2^-17), so the product with V
 // loses nothing to P's rounding; with up to 8 rows both terms share one product, above
-// the second one costs tensor time that the memory-bound loop has to spare.  Keys that no row sees are filled with zeros
-// on the way in, so what the cache holds there cannot reach the result.
+// the second one costs tensor time that the memory-bound loop has to spare.  Keys that no
+// row sees are filled with zeros on the way in, so what the cache holds there cannot reach
+// the result.
 //
 // Behind the tiled kernel of the same call it is launched programmatically: it starts on
 // SMs that have run out of tiles (the tiled kernel lets it once all of its CTAs run, when

@@ -18,7 +18,8 @@ LIB_PATH = os.path.join(_PKG, "_lib", "liblocks_b200.so")
 
 _P, _I, _L, _F, _D = c_void_p, c_int, c_int64, c_float, c_double
 
-# name -> (argtypes, kernel launches per call)
+# name -> (argtypes, kernel launches per call; locks_window_attention, which decides by its
+# sizes, takes one to three and is counted as one)
 _SIGNATURES = {
     "locks_version": ([], 0),
     "locks_set_pdl": ([_I], 0),

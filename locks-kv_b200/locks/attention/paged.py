@@ -2,6 +2,10 @@
 first tokens kept visible, and decode of a batch that shares long prefixes (host
 wrappers of ``locks_window_attention`` and ``locks_shared_prefix_decode``).
 
+A query row with a seen score of NaN or +inf becomes NaN; keys and values must be
+finite.  Weights are rounded to bf16 in the product with V where a request has more
+than 16 rows (query tokens x G) and over a shared prefix, else carried to 2^-17.
+
 Caches come in either engine layout, (NB, 2, page, n_kv, d) or (2, NB, page, n_kv, d),
 with any strides whose rows are 16-byte aligned and whose head stride is a multiple
 of 64 (a head-major view too); one of exactly two blocks is read as the latter."""
@@ -64,8 +68,8 @@ def window_paged_attention(q: torch.Tensor, kv_cache: torch.Tensor,
     ``max_q``: the query tokens of the longest request; it steers how the work is cut,
     a request with more is answered all the same, more slowly (0: nothing is done).
     ``scratch``: fp32 workspace that lets the long keys of few queries be
-    cut into parts, see :func:`attention_scratch_floats`; calls that may overlap on
-    the GPU need one each.  ``status``: int32, set where a bounded wait ran out."""
+    cut into parts, see :func:`attention_scratch_floats` (the default of two parts is
+    not enough for single tokens); calls that may overlap on the GPU need one each.  ``status``: int32, set where a bounded wait ran out."""
     dev = _cabi.one_device(q, kv_cache, block_table, cu_q, seq_lens, out, scratch, lse,
                            status)
     source, target, d, page = _checked(q, kv_cache, block_table, out, lse, scratch,
@@ -111,6 +115,7 @@ def attention_scratch_floats(n_rows: int, n_heads: int, head_dim: int = 128,
                              parts: int = 2) -> int:
     """fp32 elements that ``parts`` partial results of ``n_rows`` query tokens take
     (a maximum, a sum and ``head_dim`` values per head).  Shared-prefix decode needs
-    two; up to SMs / n_kv + 1 of them are of use to it, and up to 2 * SMs / (requests
-    * n_kv) to a windowed call with few queries over long keys."""
+    two; up to SMs / n_kv + 1 of them are of use to it.  A windowed call uses two or
+    more where a request has over 16 rows (tokens x G), and four or more, up to 2 * SMs
+    / (requests * n_kv), for single tokens and the like over 2048 pages or more."""
     return int(n_rows) * int(n_heads) * (int(head_dim) + 2) * int(parts)

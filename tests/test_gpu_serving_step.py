@@ -382,6 +382,40 @@ def test_status_of_another_type_is_refused():
         assert int(st) == 0
 
 
+def test_tables_much_wider_than_the_sequences():
+    """Tables as wide as the longest sequence allowed, entries behind the own pages that
+    name nothing, and scratch for many parts: most of them are empty."""
+    n_kv, G, reqs, W = 2, 8, [(1, 300), (40, 500), (1, 16), (2, 90)], 9000
+    lens = [l for _, l in reqs]
+    g, cache, k, v, table = paged(51, lens, n_kv)
+    wide = torch.full((4, W), -1, dtype=I32, device=DEV)
+    for r, l in enumerate(lens):
+        wide[r, :-(-l // 16)] = table[r, :-(-l // 16)]
+    scratch = torch.full((2 ** 23,), float("nan"), device=DEV)
+    cu = [0, 1, 41, 42, 44]
+    q = torch.randn(44, n_kv * G, 128, device=DEV, generator=g).to(BF16)
+    for rows in (slice(0, 4), slice(2, 4)):             # with tiles; few rows in parts
+        sub, at0 = lens[rows], cu[rows.start]
+        bounds = [c - at0 for c in cu[rows.start:]]
+        n_q = [n for n, _ in reqs[rows]]
+        lse = torch.full((bounds[-1], n_kv * G), 7.0, device=DEV)
+        out = run_window(q[at0:], cache, wide[rows], i32(bounds), i32(sub), n_kv, G, None, 0, max(n_q),
+                         lse=lse, scratch=scratch)
+        for r, l in enumerate(sub):
+            at = slice(bounds[r], bounds[r + 1])
+            check(out[at], lse[at], want_window(q[at0:][at], k, v, wide[rows][r, :-(-l // 16)], l, n_q[r],
+                                                2 ** 31 - 1, 0), r)
+    g, cache, table, lens = prefix_paged(9, [(100, [101, 160, 113]), (33, [40])], n_kv)
+    wide = torch.full((4, W), -1, dtype=I32, device=DEV)
+    for r, l in enumerate(lens):
+        wide[r, :-(-l // 16)] = table[r, :-(-l // 16)]
+    lse = torch.full((4, n_kv * G), 7.0, device=DEV)
+    out = run_prefix(q[:4], cache, wide, lens, [0, 3, 4], [100, 33], n_kv, G, lse=lse, floats=2 ** 22)
+    for r, l in enumerate(lens):
+        check(out[r:r + 1], lse[r:r + 1], want_window(q[r:r + 1], cache[:, 0], cache[:, 1], table[r], l, 1,
+                                                      2 ** 31 - 1, 0), r)
+
+
 def test_window_many_requests_few_of_them_long():
     """Several hundred requests, most with one token, prompts between them."""
     n_kv, G, R = 1, 8, 700
