@@ -33,7 +33,7 @@
 // rescaled): P stays below 2^8 and no row of O is touched in most steps.  P is rounded to
 // bf16 because V is (both operands of the product have one type), half a step each; m, l,
 // S and O are fp32.  (A second product with what the rounding left would take half again
-// as much of the tensor pipe, 64 % busy in a prompt, and twice the stores of P.)
+// as much of the tensor pipe, 63 % busy in a prompt, and twice the stores of P.)
 //
 // Every wait is bounded (status word; later waits then return at once, work and copies
 // in flight are waited for and tensor memory is freed).  No multicast.

@@ -67,9 +67,10 @@ def window_paged_attention(q: torch.Tensor, kv_cache: torch.Tensor,
     rows behind ``cu_q[R]`` stay as they were, pages that nobody sees are not read.
     ``max_q``: the query tokens of the longest request; it steers how the work is cut,
     a request with more is answered all the same, more slowly (0: nothing is done).
-    ``scratch``: fp32 workspace that lets the long keys of few queries be
-    cut into parts, see :func:`attention_scratch_floats` (the default of two parts is
-    not enough for single tokens); calls that may overlap on the GPU need one each.  ``status``: int32, set where a bounded wait ran out."""
+    ``scratch``: fp32 workspace that lets the long keys of few queries be cut into
+    parts, see :func:`attention_scratch_floats` (the default of two parts is not enough
+    for single tokens); calls that may overlap on the GPU need one each.  ``status``:
+    int32, set where a bounded wait ran out."""
     dev = _cabi.one_device(q, kv_cache, block_table, cu_q, seq_lens, out, scratch, lse,
                            status)
     source, target, d, page = _checked(q, kv_cache, block_table, out, lse, scratch,
